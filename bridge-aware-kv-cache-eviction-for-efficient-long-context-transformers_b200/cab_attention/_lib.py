@@ -32,6 +32,17 @@ _c_float = ctypes.c_float
 _c_size = ctypes.c_size_t
 _i64_3 = ctypes.c_int64 * 3
 
+class PageCache(ctypes.Structure):
+    """cab_page_cache (include/cab_capi.h): where a paged KV cache's state lives."""
+    _fields_ = [("k_pages", _c_ptr), ("v_pages", _c_ptr), ("layers", _c_i64), ("pages", _c_i64),
+                ("heads", _c_i64), ("page_size", _c_i64), ("dim", _c_i64), ("k_strides", _c_i64 * 4),
+                ("v_strides", _c_i64 * 4), ("block_table", _c_ptr), ("rows", _c_i64), ("width", _c_i64),
+                ("table_stride", _c_i64), ("seq_lens", _c_ptr), ("ref_counts", _c_ptr),
+                ("status", _c_ptr), ("dtype", _c_i64)]
+
+
+_c_cache = ctypes.POINTER(PageCache)
+
 # name -> (argtypes) ; every entry point returns int except cab_last_error_string
 SIGNATURES = {
     "cab_get_version": [],
@@ -73,6 +84,15 @@ SIGNATURES = {
                          _c_i64, _c_i64, _c_i64, _c_i64, _c_float, _c_float, _c_int, _c_int,
                          _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr, _c_size,
                          _c_ptr],
+    "cab_pages_update_workspace_size": [_c_cache, _c_i64, ctypes.POINTER(_c_size)],
+    "cab_pages_update": [_c_cache, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_int, _c_i64,
+                         _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_int, _c_ptr, _c_size, _c_ptr],
+    "cab_pages_write": [_c_cache, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr,
+                        _c_ptr, _c_i64, _c_ptr],
+    "cab_tree_attn_workspace_size": [_c_cache, _c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_size)],
+    "cab_tree_attn_fwd": [_c_cache, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr,
+                          _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_float, _c_ptr,
+                          _c_size, _c_ptr],
 }
 
 

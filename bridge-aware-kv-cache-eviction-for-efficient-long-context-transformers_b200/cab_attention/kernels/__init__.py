@@ -7,3 +7,4 @@ from .sparse_attention import block_sparse_attention  # noqa: F401
 from .frc_triton import compute_frc, compute_frc_pytorch, compute_frc_triton  # noqa: F401
 from .flash_attention_accumulate import (flash_attention_forward,  # noqa: F401
                                          flash_attention_with_cumulative_scores)
+from .tree_attention import tree_attention  # noqa: F401

@@ -12,6 +12,8 @@
 #include "prefill_host.cu"
 #include "node_frc.cu"
 #include "evict.cu"
+#include "paged_cache.cu"
+#include "tree_attn.cu"
 
 extern "C" int cab_get_version(void) { return CAB_API_VERSION; }
 

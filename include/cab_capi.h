@@ -317,6 +317,101 @@ CAB_API int cab_prefill_host(const void* q, const void* k, const void* v, void* 
                              int keep_diagonal, int causal, float softmax_scale, int dtype,
                              void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- paged KV cache
+ * A cache of `layers` layers whose K and V live in `pages` pages of `page_size` tokens:
+ * element (l, p, h, s, d) of the pages is at ptr[l*st[0] + p*st[1] + h*st[2] + s*st[3] + d].
+ * Token x of sequence row r is in slot x % page_size of page block_table[r*table_stride +
+ * x / page_size]; entries past a row's pages are -1. ref_counts[p] rows use page p (0: free).
+ * A page whose content ends inside it is used by one row alone. `status` is one word that
+ * collects CAB_PAGES_* bits: while it is not 0, updates and writes do nothing.
+ * The reference keeps one contiguous tensor per layer and rebuilds it to evict
+ * (cab_attention/cache/cab_cache.py:122-226); this form has no counterpart there.
+ */
+typedef struct cab_page_cache {
+  void* k_pages;
+  void* v_pages;
+  int64_t layers, pages, heads, page_size, dim;
+  int64_t k_strides[4], v_strides[4]; /* {layer, page, head, slot} in elements, positive */
+  int32_t* block_table;               /* [rows, width] */
+  int64_t rows, width, table_stride;
+  int32_t* seq_lens;   /* [rows] */
+  int32_t* ref_counts; /* [pages] */
+  int32_t* status;     /* [1] */
+  int64_t dtype;
+} cab_page_cache;
+
+#define CAB_PAGES_FULL 1       /* not enough free pages                                       */
+#define CAB_PAGES_TABLE_FULL 2 /* a row would hold more tokens than its table has pages for   */
+#define CAB_PAGES_BAD_ROW 4    /* a row outside [0, rows), or written twice by one call       */
+#define CAB_PAGES_BAD_ARG 8    /* a length, count or kept position out of range               */
+#define CAB_PAGES_BAD_TABLE 16 /* a page number outside [0, pages), or a shared last page     */
+
+/* Scratch bytes cab_pages_update needs for n pairs. */
+CAB_API int cab_pages_update_workspace_size(const cab_page_cache* cache, int64_t n, size_t* bytes);
+
+/*
+ * For n pairs of rows (src[i], dst[i]) at once: row dst[i] becomes the first start[i] tokens
+ * of src[i], then its tokens at start[i] + keep[i*keep_stride + x] for x < keep_num[i]
+ * (< keep_cols), then room for grow[i] tokens (not written). All reads are of the state
+ * before the call, so a row may be the source of others and be overwritten. With
+ * dst[i] == src[i] it is compaction or truncation in place (start 0, no list: the row is
+ * freed), otherwise dst[i]'s pages are given up first. Pages whose tokens stay in place are
+ * shared between rows; the others come from the lowest-numbered free pages in order of i, and
+ * pages given up by a call are free from the next call on.
+ * Arrays may be NULL: src (0 .. n-1), dst (src), start (start_value; < 0: the whole length),
+ * keep_num (keep_cols), grow (grow_value). keep is int32 or int64 (keep_bytes 4 or 8), any
+ * order; keep_num has a stride. A row may be written once per call; n <= 1024.
+ * copies == 0: for calls that only lengthen rows or free them: no list, and no last page may
+ * need a copy (k_pages / v_pages are not touched). All or nothing: on a device-side refusal
+ * only the status word changes.
+ * Applies the eviction that CABCache._evict makes (cab_attention/cache/cab_cache.py:177-226).
+ */
+CAB_API int cab_pages_update(const cab_page_cache* cache, const int32_t* src, const int32_t* dst,
+                             int64_t n, const int32_t* start, int64_t start_value,
+                             const void* keep, int keep_bytes, int64_t keep_stride,
+                             int64_t keep_cols, const int32_t* keep_num, int64_t keep_num_stride,
+                             const int32_t* grow, int64_t grow_value, int copies, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/*
+ * Writes k, v [n,Hkv,T,D] (strides {n, h, t}, any non-negative) into one layer: token t of
+ * sequence i, t < num_new[i] (NULL: num_value), becomes token seq_len - num_new[i] + t of row
+ * rows[i] (NULL: i). Rows must differ.
+ */
+CAB_API int cab_pages_write(const cab_page_cache* cache, int64_t layer, const void* k,
+                            const void* v, int64_t n, int64_t T, const int64_t* k_strides,
+                            const int64_t* v_strides, const int32_t* rows, const int32_t* num_new,
+                            int64_t num_value, void* stream);
+
+/* Scratch bytes cab_tree_attn_fwd needs. */
+CAB_API int cab_tree_attn_workspace_size(const cab_page_cache* cache, int64_t n, int64_t Hq,
+                                         int64_t T, size_t* bytes);
+
+/*
+ * Attention of n sequences' newest tokens over their cache: q, out [n,Hq,T,D] with strides
+ * {n, h, t}. Sequence i is row rows[i] (NULL: i); its last m = num_nodes[i] (NULL: T) cached
+ * tokens are its nodes, whose queries are q[i, :, :m]. A node sees every earlier token of the
+ * cache and, among the nodes, its ancestors and itself (parents [n,T] with row stride
+ * parents_stride, 0 = one tree for all; parents[t] < t, negative: a root), or those with
+ * tree_mask[i,t,u] != 0 (uint8 [n,T,T], stride mask_stride, 0 = one mask), or u <= t when
+ * both are NULL. softmax over the seen tokens; a query that sees none and the queries past m
+ * give 0 (lse -inf). lse [n,Hq,T] fp32 natural log, may be NULL. A sequence whose row is out
+ * of range, whose m exceeds its length, or a page outside [0, pages) is not read: its output
+ * is that of a query that sees none, or leaves out the page's tokens.
+ * bf16 / f16 with head_dim 64 or 128 and page_size 8, 16, 32, 64 or a multiple of 128 run on
+ * the tensor cores (pages 16-byte aligned); other head_dim <= 256, page sizes and float32 on
+ * CUDA cores.
+ * Extends flash_attention_with_cumulative_scores' KV-cache steps
+ * (cab_attention/kernels/flash_attention_accumulate.py:169-261) to pages and trees.
+ */
+CAB_API int cab_tree_attn_fwd(const cab_page_cache* cache, int64_t layer, const void* q, void* out,
+                              float* lse, int64_t n, int64_t Hq, int64_t T,
+                              const int64_t* q_strides, const int64_t* o_strides,
+                              const int32_t* rows, const int32_t* num_nodes,
+                              const int32_t* parents, int64_t parents_stride,
+                              const uint8_t* tree_mask, int64_t mask_stride, float softmax_scale,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
