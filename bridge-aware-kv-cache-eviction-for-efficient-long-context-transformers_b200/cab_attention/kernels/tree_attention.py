@@ -130,7 +130,7 @@ def attend_cache(cache, device, dtype, layer: int, q: torch.Tensor, parents=None
     if n == 0 or T == 0:
         return (out, lse) if return_lse else out
     es = q.element_size()
-    if q.stride(3) != 1 or any((s * es) % 16 for s in q.stride()[:3]) or q.data_ptr() % 16:
+    if q.stride(3) != 1 or any(s <= 0 or (s * es) % 16 for s in q.stride()[:3]) or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)  # contiguous() would return a misaligned dense view
     L = _lib.lib()
     with on_device(device):

@@ -56,6 +56,7 @@ struct Params {
   int32_t least;      // tensor-core path: tiles a CTA takes at least
   int32_t part_rows;  // rows of a partial slot
   int32_t out_vec;    // out rows start on 16 bytes
+  int32_t whole_units;  // no unit is cut: none can be longer than a few tiles
   float *part_o, *part_ml;
 };
 
@@ -276,166 +277,180 @@ __global__ void __launch_bounds__(kSimtThreads) simt_join_kernel(const Params p)
 }
 
 // ------------------------------------------------------------------ tensor-core path
-// bf16 / f16, head_dim 64 or 128. A unit is (sequence, KV head, row group); a row group is up
-// to 128 rows (kDual false) or 256 (kDual true) of the G * T rows that share the head's keys. The
-// units' 128-key tiles form one flat list that is cut into equal ranges, one per CTA
-// (persistent, one CTA per SM), so ragged lengths balance and a single long sequence fills the
-// GPU; a unit cut between CTAs leaves partial sums that join_kernel adds in key order.
+// bf16 / f16, head_dim 64 or 128. The G * T rows of a (sequence, KV head) are cut into groups
+// of whole nodes, at most 128 rows, the M of tcgen05.mma. Up to kMaxShare groups are worked on side by side by as many CTAs, so
+// that a K / V tile comes from HBM once and for the others from L2. A unit is (sequence, KV head, such a
+// set of groups); the units' 128-key tiles form one flat list that is cut into equal ranges, one
+// per set of CTAs (persistent, one CTA per SM), so ragged lengths balance and one long sequence
+// fills the GPU; a unit cut between ranges leaves partial sums that join_kernel adds in key order.
 //
-// Two streams of work share the tensor pipe, so one's softmax runs under the other's products:
-// with kDual the two 128-row halves of the group against the same K/V tile; else the even and
-// the odd key tiles of one 128-row group, each with its own O, maximum and sum, merged at the
-// end of the range. Stream s, its tile i:
-//   S = Q K^T (tcgen05.mma, 128 x 128, K-major from shared memory) -> 128 TMEM columns,
-//   p = 2^(s - m) by four warps, one thread per row, written as 16-bit over the S columns
-//   (the products' operand type; its sum is taken before the rounding, in float32),
-//   O += P V (P from TMEM, V MN-major from its natural layout).
-// One thread issues all products in the order PV(i), S(i + 1) per stream, so completion of S(i + 1)
-// implies that of PV(i): O may be rescaled then (only when the maximum has grown by more than
-// 2^8), and S(i + 1) may overwrite P(i).
+// Tile g of a CTA: S = Q K^T (128 x 128, K-major operands from shared memory) into one of three
+// TMEM buffers; p = 2^(s - m) by two threads per row (64 keys each, which swap their maxima through
+// shared memory), written over S as 16-bit, the products' operand type (its sum is taken before
+// that rounding, in float32); O += P V (P from TMEM, V MN-major as it lies in the pages). S(g + 3) reuses
+// the buffer once PV(g) has completed. O is rescaled only when the maximum has grown by more than 2^8.
 //
-// Warp 0 looks up the pages and loads K and V tiles by TMA (one box per page and 64 columns)
-// through one ring of stages; a page number outside the pool reads zeros. Tiles that reach into the nodes
-// or past the length are masked per row by a 128-bit word, and the unused or unseen rows of V that are not
-// finite are zeroed in shared memory, so that 0 * NaN cannot enter a product; a seen value that is not
-// finite is added back to the rows that see it (fix_up).
+// Warps 0 and 3 look up the pages and load K and V by TMA (one box per page and 64 columns, a lane
+// each; a page number outside the pool reads zeros), so loads are issued from two warps (one warp
+// gives 5.3 TB/s with 16-token pages, two 5.9, copy peak 6.55). Tiles that reach into the nodes or past the
+// length are masked per row by a 64-bit word, and V rows past the length and values of nodes that
+// are not finite are zeroed in shared memory, so that 0 * NaN cannot enter a product; a seen value
+// that is not finite is added back to the rows that see it (fix_up).
+//
+// Every mbarrier has one waiter per phase and direction, or its next phase needs the waiter's own
+// next step, so parity waits never meet a barrier two phases on.
 
-constexpr int kTcThreads = 384;  // warp 0: TMA, warp 1: products, warps 4-7 / 8-11: streams 0 / 1
+constexpr int kTcThreads = 384;  // warps 0 / 3: K / V loads, 1: S, 2: PV, 4-11: softmax and epilogue
 constexpr float kRescaleThreshold = 8.0f;
-constexpr uint32_t kTmemO = 256;
+constexpr int kBufs = 3;
+constexpr uint32_t kTmemO = 384;
+constexpr int kMaxShare = 4;
+constexpr int kWholeTiles = 4;  // rows of at most this many tiles are not cut: no join
 
-template <int D, bool kDual>
+template <int D>
 struct Cfg {
   static constexpr int kTile = 128 * D * 2;  // bytes of a K, V or Q tile
   static constexpr int kAtoms = D / 64;
-  static constexpr int kQTiles = kDual ? 2 : 1;
-  static constexpr int kRows = 128 * kQTiles;
-  static constexpr int kStages = (7 - kQTiles) * (D == 64 ? 2 : 1);
-  static constexpr int kBars = (2 * kStages + 8) * 8 + 64;
-  static constexpr int kSmem = kQTiles * kTile + kStages * kTile + kBars + 1024;
-  static_assert(kSmem <= 232448, "shared memory");
+  static constexpr int kStages = D == 128 ? 3 : 6;  // of K, and of V
+  // with as many stages as S / P buffers S(g) completed frees K stage g % 3, PV(g) V stage g % 3
+  static constexpr bool kOneSignal = kStages == kBufs;
+  static constexpr int kXchg = 2 * 2 * 128 * 4;  // row maxima / sums [parity][key half][row]
+  static constexpr int kBars = (4 * kStages + 3 * kBufs + 3) * 8 + 32;
+  static constexpr int kBytes = (1 + 2 * kStages) * kTile + kXchg + kBars;
+  static constexpr int kSmem = kBytes + 1024 < 232448 ? kBytes + 1024 : 232448;  // the kernel checks that it fits
+  static_assert(kBytes <= 232448, "shared memory");
 };
 
-struct Walk {  // a range of the flat tile list, unit by unit
-  int b, hk, grp, tiles, at;  // tile `at` of `tiles`
-  int left;                   // tiles of the range not yet walked
+// How the nodes are shared out: groups of `nodes` whole nodes (their G rows each, at most 128 rows), `wide`
+// groups side by side, `sets` of them per KV head.
+struct Share {
+  int nodes, groups, wide, sets;
+};
+__host__ __device__ __forceinline__ Share share_of(int G, int T) {
+  Share s;
+  s.nodes = 128 / G;
+  s.groups = (T + s.nodes - 1) / s.nodes;
+  s.sets = (s.groups + kMaxShare - 1) / kMaxShare;
+  s.wide = (s.groups + s.sets - 1) / s.sets;
+  return s;
+}
+
+struct Walk {  // a range of the flat list, unit by unit
+  int b, hk, set, tiles, at;  // tile `at` of the unit's `tiles`
+  int left;                   // tiles (units, where units stay whole) of the range not yet walked
   Seq s;
 };
 
-template <int kRows>
-__device__ __forceinline__ int unit_keys(const Params& p, const Seq& s, int grp) {
-  const int t0 = grp * kRows / p.G;
-  return t0 < s.m ? key_limit(p, s, min(p.T - 1, (grp * kRows + kRows - 1) / p.G)) : 0;
+// Keys that groups [g0, g1] of sequence s can see, 0 where none of their rows is a node.
+__device__ __forceinline__ int group_keys(const Params& p, const Share& sh, const Seq& s, int g0, int g1) {
+  return g0 * sh.nodes < s.m ? key_limit(p, s, min(p.T, (g1 + 1) * sh.nodes) - 1) : 0;
 }
-template <int kRows>
-__device__ __forceinline__ int unit_tiles(const Params& p, const Seq& s, int grp) {
-  return max(1, (unit_keys<kRows>(p, s, grp) + 127) / 128);
+__device__ __forceinline__ int tiles_of(int keys) { return max(1, (keys + 127) / 128); }  // at least one, for the zeros
+__device__ __forceinline__ int unit_tiles(const Params& p, const Share& sh, const Seq& s, int set) {
+  return tiles_of(group_keys(p, sh, s, set * sh.wide, min(sh.groups, (set + 1) * sh.wide) - 1));
 }
-template <int kRows>
-__device__ __forceinline__ int seq_tiles(const Params& p, const Seq& s) {  // of one KV head
-  const int groups = (p.G * p.T + kRows - 1) / kRows;
+// What a unit counts in the flat list, and the units of one KV head of a sequence.
+__device__ __forceinline__ int unit_weight(const Params& p, const Share& sh, const Seq& s, int set) {
+  return p.whole_units ? 1 : unit_tiles(p, sh, s, set);
+}
+__device__ __forceinline__ int head_weight(const Params& p, const Share& sh, const Seq& s) {
+  if (p.whole_units) return sh.sets;
   int sum = 0;
-  for (int g = 0; g < groups; ++g) sum += unit_tiles<kRows>(p, s, g);
+  for (int g = 0; g < sh.sets; ++g) sum += unit_tiles(p, sh, s, g);
   return sum;
 }
 
-template <int kRows>
-__device__ __forceinline__ void walk_next(const Params& p, Walk& w) {  // to the next unit's first tile
-  const int groups = (p.G * p.T + kRows - 1) / kRows;
-  w.left -= min(w.left, w.tiles - w.at);
+__device__ __forceinline__ void walk_next(const Params& p, const Share& sh, Walk& w) {  // to the next unit's first tile
+  w.left -= p.whole_units ? 1 : min(w.left, w.tiles - w.at);
   w.at = 0;
-  if (++w.grp == groups) {
-    w.grp = 0;
+  if (w.left == 0) return;
+  if (++w.set == sh.sets) {
+    w.set = 0;
     if (++w.hk == p.Hkv) {
       w.hk = 0;
-      ++w.b;
-      if (w.left > 0) w.s = load_seq(p, w.b);
+      w.s = load_seq(p, ++w.b);
     }
   }
-  if (w.left > 0) w.tiles = unit_tiles<kRows>(p, w.s, w.grp);
+  w.tiles = unit_tiles(p, sh, w.s, w.set);
+}
+// Tiles of the walk's segment that group grp works on (the unit's longest group has them all).
+__device__ __forceinline__ int own_tiles(const Params& p, const Share& sh, const Walk& w, int grp) {
+  if (grp >= sh.groups) return 0;
+  const int end = min(w.tiles, tiles_of(group_keys(p, sh, w.s, grp, grp)));
+  return max(0, (p.whole_units ? end : min(end, w.at + w.left)) - w.at);
 }
 
-__host__ __device__ __forceinline__ int64_t range_start(int64_t total, int64_t ctas, int64_t c) { return total * c / ctas; }
-__device__ __forceinline__ int range_ctas(int64_t total, int ctas, int least) {
-  return static_cast<int>(min(static_cast<int64_t>(ctas), (total + least - 1) / least));
+__host__ __device__ __forceinline__ int64_t range_start(int64_t total, int64_t ranges, int64_t c) { return total * c / ranges; }
+__device__ __forceinline__ int range_count(int64_t total, int most, int least) {
+  return static_cast<int>(min(static_cast<int64_t>(most), (total + least - 1) / least));
 }
 
-// Warp-wide: the total number of tiles, and the sequence that holds flat tile `f` with the tiles before it.
-template <int kRows>
-__device__ __forceinline__ int64_t total_tiles(const Params& p) {
+// Warp-wide: the weight of all units and, if `count` is not 0, of this range: the sequence in which its
+// first unit lies, the weight before that sequence, and the range's own.
+__device__ __forceinline__ int64_t total_weight(const Params& p, const Share& sh) {
   const int lane = threadIdx.x & 31;
   int64_t sum = 0;
-  for (int b = lane; b < p.n; b += 32) sum += static_cast<int64_t>(seq_tiles<kRows>(p, load_seq(p, b))) * p.Hkv;
+  for (int b = lane; b < p.n; b += 32) sum += static_cast<int64_t>(head_weight(p, sh, load_seq(p, b))) * p.Hkv;
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;
 }
-template <int kRows>
-__device__ __forceinline__ void find_seq(const Params& p, int64_t f, int* b_out, int64_t* before) {
+struct Begin {
+  int b, offset, left;
+};
+__device__ __forceinline__ Begin find_range(const Params& p, const Share& sh, int range, int most) {
   const int lane = threadIdx.x & 31;
+  const int64_t total = total_weight(p, sh);
+  const int ranges = range_count(total, most, p.least);
+  if (range >= ranges) return Begin{0, 0, 0};
+  const int64_t f0 = range_start(total, ranges, range), f1 = range_start(total, ranges, range + 1);
   int64_t base = 0;
   for (int b0 = 0; b0 < p.n; b0 += 32) {
-    const int b = b0 + lane;
-    const int64_t own = b < p.n ? static_cast<int64_t>(seq_tiles<kRows>(p, load_seq(p, b))) * p.Hkv : 0;
+    const int b = b0 + lane;  // the second reading of the lengths hits L1
+    const int64_t own = b < p.n ? static_cast<int64_t>(head_weight(p, sh, load_seq(p, b))) * p.Hkv : 0;
     int64_t inc = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += u;
     }
-    const uint32_t hit = __ballot_sync(0xffffffffu, base + inc > f);
+    const uint32_t hit = __ballot_sync(0xffffffffu, base + inc > f0);
     if (hit) {
       const int l = __ffs(hit) - 1;
-      *b_out = b0 + l;
-      *before = base + __shfl_sync(0xffffffffu, inc - own, l);
-      return;
+      return Begin{b0 + l, static_cast<int>(f0 - base - __shfl_sync(0xffffffffu, inc - own, l)), static_cast<int>(f1 - f0)};
     }
     base += __shfl_sync(0xffffffffu, inc, 31);
   }
-  *b_out = p.n - 1;
-  *before = base;
+  return Begin{0, 0, 0};
 }
 
-struct Bits {
-  uint64_t lo, hi;
-};
 __device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
-// Which of the keys key0 .. key0 + 127 node t of sequence b sees.
-__device__ __noinline__ Bits seen_bits(const Params& p, const Seq& s, int b, int t, int key0, bool bad_pages) {
+// Which of the keys key0 .. key0 + 63 node t of sequence b sees.
+__device__ __noinline__ uint64_t seen_bits(const Params& p, const Seq& s, int b, int t, int key0, bool bad_pages) {
   const int c = s.ctx - key0;
-  Bits w{low_bits(c), low_bits(c - 64)};
+  uint64_t w = low_bits(c);
   if (p.parents) {
     const int32_t* up = p.parents + b * p.parents_stride;
     for (int x = t; x >= 0;) {
       const int at = c + x;
       if (at < 0) break;
-      if (at < 64) w.lo |= 1ull << at;
-      else if (at < 128) w.hi |= 1ull << (at - 64);
+      if (at < 64) w |= 1ull << at;
       const int y = up[x];
       if (y >= x) break;
       x = y;
     }
   } else if (p.mask) {
     const uint8_t* row = p.mask + b * p.mask_stride + static_cast<int64_t>(t) * p.T;
-    for (int at = max(c, 0); at < min(128, c + s.m); ++at)
-      if (row[at - c]) {
-        if (at < 64) w.lo |= 1ull << at;
-        else w.hi |= 1ull << (at - 64);
-      }
+    for (int at = max(c, 0); at < min(64, c + s.m); ++at)
+      if (row[at - c]) w |= 1ull << at;
   } else {
-    w.lo = low_bits(c + t + 1);
-    w.hi = low_bits(c + t + 1 - 64);
+    w = low_bits(c + t + 1);
   }
   if (bad_pages) {
-    for (int j = 0; j < 128; ++j) {
-      const int key = key0 + j;
-      if (key >= s.len) break;
-      const int pg = p.table[s.row * p.table_stride + key / p.page_size];
-      if (pg < 0 || pg >= p.pages) {
-        if (j < 64) w.lo &= ~(1ull << j);
-        else w.hi &= ~(1ull << (j - 64));
-      }
+    for (int j = 0; j < 64 && key0 + j < s.len; ++j) {
+      const int pg = p.table[s.row * p.table_stride + (key0 + j) / p.page_size];
+      if (pg < 0 || pg >= p.pages) w &= ~(1ull << j);
     }
   }
   return w;
@@ -457,32 +472,31 @@ __device__ __noinline__ void fix_up(const Params& p, const Seq& s, int b, int hk
   }
 }
 
-// Row `r` of a V tile: beyond the length it becomes 0; of a node, elements that are not finite do.
-// Returns whether there were any.
+// Half `half` (D / 2 columns) of row r of a V tile: past the length it becomes 0; of a node, elements
+// that are not finite do. Returns whether there were any.
 template <int D, bool kBF16>
-__device__ __forceinline__ bool clean_v_row(uint8_t* tile, int r, int key, const Seq& s) {
+__device__ __forceinline__ bool clean_v_row(uint8_t* tile, int r, int half, int key, const Seq& s) {
   constexpr uint32_t kExp = kBF16 ? 0x7F80u : 0x7C00u;
   bool found = false;
 #pragma unroll
-  for (int a = 0; a < D / 64; ++a)
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      uint4* q = reinterpret_cast<uint4*>(tile + a * 16384 + sw128_offset(r, c));
-      if (key >= s.len) {
-        *q = make_uint4(0, 0, 0, 0);
-        continue;
-      }
-      uint4 x = *q;
-      uint32_t* e = reinterpret_cast<uint32_t*>(&x);
-      bool hit = false;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if ((e[k] & kExp) == kExp) { e[k] &= 0xFFFF0000u; hit = true; }
-        if ((e[k] & (kExp << 16)) == (kExp << 16)) { e[k] &= 0x0000FFFFu; hit = true; }
-      }
-      if (hit) *q = x;
-      found |= hit;
+  for (int c = 0; c < D / 16; ++c) {
+    const int x = half * (D / 16) + c;  // 16-byte chunk of the row
+    uint4* q = reinterpret_cast<uint4*>(tile + (x >> 3) * 16384 + sw128_offset(r, x & 7));
+    if (key >= s.len) {
+      *q = make_uint4(0, 0, 0, 0);
+      continue;
     }
+    uint4 v = *q;
+    uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+    bool hit = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if ((e[k] & kExp) == kExp) { e[k] &= 0xFFFF0000u; hit = true; }
+      if ((e[k] & (kExp << 16)) == (kExp << 16)) { e[k] &= 0x0000FFFFu; hit = true; }
+    }
+    if (hit) *q = v;
+    found |= hit;
+  }
   return found;
 }
 
@@ -497,85 +511,127 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-__device__ __forceinline__ bool streams_sync_or(bool x) {  // the 256 threads of both streams
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\t"
-      "barrier.cta.red.or.pred b, 1, 256, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
-      : "=r"(r)
-      : "r"(static_cast<uint32_t>(x))
-      : "memory");
-  return r != 0;
+__device__ __forceinline__ void softmax_sync() {  // the 256 threads of the softmax warps
+  asm volatile("barrier.cta.sync 5, 256;" ::: "memory");
 }
-__device__ __forceinline__ void streams_sync() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void pair_sync(int quad) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(1 + quad) : "memory"); }
 
-// Places in a range's ring sequence of a segment of T tiles: K(0) K(1) V(0) K(2) V(1) ... (single),
-// K(0) V(0) K(1) V(1) ... (dual), in the order in which the products need them.
-template <bool kDual>
-__device__ __forceinline__ uint32_t place_k(int g) {
-  return kDual ? 2 * g : (g == 0 ? 0 : 2 * g - 1);
+__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n\t"
+      "mov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
-template <bool kDual>
-__device__ __forceinline__ uint32_t place_v(int g, int T) {
-  return kDual ? 2 * g + 1 : (g == T - 1 ? 2 * T - 1 : 2 * g + 2);
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rd, ra, rb;\n\t"
+      "mov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
-template <int D, bool kBF16, bool kDual>
+// Up to 64 weights of a row's half tile from its scores s[64] (in place), kMasked: only those of
+// the bits `see`. Writes P and returns their sum.
+template <bool kBF16, bool kMasked>
+__device__ __forceinline__ float weights(uint32_t (&s)[64], uint64_t see, float scale, float sub, uint32_t t_p) {
+  const float2 sc = make_float2(scale, scale), nm = make_float2(-sub, -sub);
+  float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t word = static_cast<uint32_t>(see >> (32 * h));
+    uint32_t y[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int c = 32 * h + 2 * k;
+      const float2 x = ffma2(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc, nm);
+      float p0 = ex2(x.x), p1 = ex2(x.y);
+      if constexpr (kMasked) {
+        p0 = word >> (2 * k) & 1u ? p0 : 0.f;
+        p1 = word >> (2 * k + 1) & 1u ? p1 : 0.f;
+      }
+      acc[k & 1] = fadd2(acc[k & 1], make_float2(p0, p1));
+      y[k] = pack2<kBF16>(p0, p1);
+    }
+    tmem_st16(t_p + 16 * h, y);
+  }
+  return (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+}
+
+template <int D, bool kBF16>
 __global__ void __launch_bounds__(kTcThreads, 1)
     tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-              const __grid_constant__ Params p) {
-  using C = Cfg<D, kDual>;
+              const __grid_constant__ CUtensorMap qmap, const __grid_constant__ Params p) {
+  using C = Cfg<D>;
   using InT = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
-  constexpr int kRows = C::kRows, kStages = C::kStages;
+  constexpr int kStages = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = base;
-  uint8_t* ring = sQ + C::kQTiles * C::kTile;
-  uint64_t* kv_full = reinterpret_cast<uint64_t*>(ring + kStages * C::kTile);
-  uint64_t* kv_empty = kv_full + kStages;
-  uint64_t* s_full = kv_empty + kStages;  // [2] S of stream s is there (and its earlier PV done)
-  uint64_t* p_full = s_full + 2;          // [2] P of stream s is there (4 warps)
-  uint64_t* q_full = p_full + 2;          // Q of the segment is there (8 warps)
-  uint64_t* drain = q_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint8_t* sK = sQ + C::kTile;
+  uint8_t* sV = sK + kStages * C::kTile;
+  float* xchg = reinterpret_cast<float*>(sV + kStages * C::kTile);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(xchg + C::kXchg / 4);
+  uint64_t* v_full = k_full + kStages;
+  uint64_t* k_empty = v_full + kStages;    // unused with kOneSignal
+  uint64_t* v_empty = k_empty + kStages;   // unused with kOneSignal
+  uint64_t* s_full = v_empty + kStages;    // [3] S(g) is there
+  uint64_t* p_full = s_full + kBufs;       // [3] P(g) is there (8 warps)
+  uint64_t* buf_free = p_full + kBufs;     // [3] PV(g) has completed
+  uint64_t* q_full = buf_free + kBufs;     // Q of the segment is there
+  uint64_t* drain = q_full + 1;            // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  int* odd_flag = abort_flag + 1;  // a V tile of the segment held values that are not finite
-  int* s_begin = odd_flag + 1;     // first sequence, KV head, group, tile; tiles of the range; flat start
+  int* odd_seg = abort_flag + 1;   // the last segment (from 1) whose V tiles held values that are not finite
+  int* begin = odd_seg + 1;        // the range: first sequence, weight before it in there, own weight
+  {
+    uint32_t dyn;
+    asm volatile("mov.u32 %0, %%dynamic_smem_size;" : "=r"(dyn));
+    if (base + C::kBytes > smem_raw + dyn) {
+      if (threadIdx.x == 0) atomicOr(&g_device_status, CAB_DEVICE_LAYOUT);
+      return;  // shared memory does not start where expected: nothing was touched
+    }
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Share sh = share_of(p.G, p.T);
+  const int range = blockIdx.x / sh.wide, side = blockIdx.x % sh.wide;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 32) {
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
-    }
-    for (int s = 0; s < 2; ++s) {
+    prefetch_tensormap(&qmap);
+    for (int s = 0; s < 4 * kStages; ++s) mbar_init(&k_full[s], 1);
+    for (int s = 0; s < kBufs; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
+      mbar_init(&p_full[s], 8);
+      mbar_init(&buf_free[s], 1);
     }
-    mbar_init(q_full, 8);
-    mbar_init(drain, 1);
+    mbar_init(q_full, 1);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     *abort_flag = 0;
-    *odd_flag = 0;
+    *odd_seg = 0;
     fence_barrier_init();
   }
   if (warp == 2) tmem_alloc(tmem_slot, 512);
   if (warp == 0) {
-    const int64_t total = total_tiles<kRows>(p);
-    const int ctas = range_ctas(total, gridDim.x, p.least);
-    int64_t f0 = 0, f1 = 0, before = 0;
-    int b = 0;
-    if (static_cast<int>(blockIdx.x) < ctas) {
-      f0 = range_start(total, ctas, blockIdx.x);
-      f1 = range_start(total, ctas, blockIdx.x + 1);
-      find_seq<kRows>(p, f0, &b, &before);
-    }
+    const Begin x = find_range(p, sh, range, gridDim.x / sh.wide);
     if (lane == 0) {
-      s_begin[0] = b;
-      s_begin[1] = static_cast<int>(f0 - before);
-      s_begin[2] = static_cast<int>(f1 - f0);
+      begin[0] = x.b;
+      begin[1] = x.offset;
+      begin[2] = x.left;
     }
   }
   tc_fence_before_sync();
@@ -584,225 +640,226 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t tmem = *tmem_slot;
 
   Walk w;
-  w.b = s_begin[0];
-  w.left = s_begin[2];
-  w.hk = w.grp = w.at = 0;
+  w.b = begin[0];
+  w.left = begin[2];
+  w.hk = w.set = w.at = 0;
   w.tiles = 1;
   if (w.left > 0) {
     w.s = load_seq(p, w.b);
-    const int per_head = seq_tiles<kRows>(p, w.s);
-    int rem = s_begin[1];
+    const int per_head = head_weight(p, sh, w.s);
+    int rem = begin[1];
     w.hk = rem / per_head;
     rem -= w.hk * per_head;
-    for (w.tiles = unit_tiles<kRows>(p, w.s, 0); rem >= w.tiles; w.tiles = unit_tiles<kRows>(p, w.s, ++w.grp)) rem -= w.tiles;
+    while (rem >= unit_weight(p, sh, w.s, w.set)) rem -= unit_weight(p, sh, w.s, w.set++);
+    w.tiles = unit_tiles(p, sh, w.s, w.set);
     w.at = rem;
   }
 
-  if (warp == 0) {
-    // ---------------------------------------------------------------- TMA producer
+  if (warp == 0 || warp == 3) {
+    // ---------------------------------------------------------------- loads: warp 0 K, warp 3 V
+    const bool is_k = warp == 0;
+    const CUtensorMap* map = is_k ? &kmap : &vmap;
+    uint8_t* ring = is_k ? sK : sV;
+    uint64_t* full = is_k ? k_full : v_full;
+    uint64_t* empty = C::kOneSignal ? (is_k ? s_full : buf_free) : (is_k ? k_empty : v_empty);
     const int S = static_cast<int>(p.page_size);
     const int per_tile = S < 128 ? 128 / S : 1;
     const int pi = lane / C::kAtoms, a = lane % C::kAtoms;
     const bool mine = pi < per_tile;
     const uint32_t off = a * 16384 + pi * (S < 128 ? S * 128 : 0);
-    uint32_t pos = 0;
+    uint32_t g = 0, nq = 0;
     bool ok = true;
-    for (; w.left > 0 && ok; walk_next<kRows>(p, w)) {
-      const int T = min(w.left, w.tiles - w.at);
+    for (; w.left > 0 && ok; walk_next(p, sh, w)) {
+      const int T = own_tiles(p, sh, w, w.set * sh.wide + side);
+      if (T == 0) continue;
       const int held = (w.s.len + S - 1) / S;
       const int32_t* row = p.table + w.s.row * p.table_stride;
-      // the page of this lane's box in tile g of the segment (the number past the pool: zeros)
-      auto page_of = [&](int g) -> int {
-        const int j = (w.at + g) * 128 / S + (S < 128 ? pi : 0);
-        if (!mine || g >= T || j >= held) return static_cast<int>(p.pages);
+      // the page of this lane's box in tile i of the segment (the number past the pool: zeros)
+      auto page_of = [&](int i) -> int {
+        const int j = (w.at + i) * 128 / S + (S < 128 ? pi : 0);
+        if (!mine || i >= T || j >= held) return static_cast<int>(p.pages);
         const int q = row[j];
         return q < 0 || q >= p.pages ? static_cast<int>(p.pages) : q;
       };
-      auto load = [&](const CUtensorMap* map, int g, int page) {
-        const int st = pos % kStages;
-        ok = ok && mbar_wait(&kv_empty[st], ((pos / kStages) & 1) ^ 1, abort_flag);
+      int e0 = page_of(0), e1 = page_of(1);  // read two tiles ahead
+      if (is_k) {
+        // Q, once the previous segment's last S, its reader, has completed (S runs ahead of the
+        // softmax, so the next segment's first S is done by the time the softmax gets there)
+        if (g > 0) ok = mbar_wait(&s_full[(g - 1) % kBufs], ((g - 1) / kBufs) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) return;
-        if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], C::kTile);
-        __syncwarp();
-        const int slot = S < 128 ? 0 : (w.at + g) * 128 % S;
-        if (mine) tma_load_4d(ring + st * C::kTile + off, map, &kv_full[st], 64 * a, slot, w.hk, page);
-        ++pos;
-      };
-      int e0 = page_of(0), e1 = page_of(1), e2 = page_of(2);
-      if constexpr (!kDual) {
-        load(&kmap, 0, e0);
-        if (T > 1) load(&kmap, 1, e1);
-      }
-      for (int g = 0; g < T; ++g) {
-        const int e3 = page_of(g + 3);
-        if constexpr (kDual) {
-          load(&kmap, g, e0);
-          load(&vmap, g, e0);
-        } else {
-          load(&vmap, g, e0);
-          if (g + 2 < T) load(&kmap, g + 2, e2);
+        if (!ok) break;
+        ++nq;
+        if (lane == 0) {
+          const int nodes = min(sh.nodes, p.T);
+          mbar_arrive_expect_tx(q_full, nodes * p.G * D * 2);
+#pragma unroll
+          for (int k = 0; k < C::kAtoms; ++k)
+            tma_load_5d(sQ + k * 16384, &qmap, q_full, 64 * k, 0, (w.set * sh.wide + side) * sh.nodes, w.hk, w.b);
         }
+        __syncwarp();
+      }
+      for (int i = 0; i < T; ++i, ++g) {
+        const int e2 = page_of(i + 2);
+        const uint32_t st = g % kStages;
+        // tile g - kStages, the stage's last reader, has completed
+        ok = mbar_wait(&empty[st], ((g / kStages) & 1) ^ 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], C::kTile);
+        __syncwarp();
+        if (mine) tma_load_4d(ring + st * C::kTile + off, map, &full[st], 64 * a, S < 128 ? 0 : (w.at + i) * 128 % S, w.hk, e0);
+        __syncwarp();
         e0 = e1;
         e1 = e2;
-        e2 = e3;
       }
     }
     if (!ok) {  // copies still in flight land before the CTA ends
-      for (uint32_t k = 0; k < kStages && k < pos; ++k) {
-        const uint32_t q = pos - 1 - k;
-        (void)mbar_wait(&kv_full[q % kStages], (q / kStages) & 1, nullptr);
-      }
+      for (uint32_t k = 1; k <= kStages && k <= g; ++k) (void)mbar_wait(&full[(g - k) % kStages], ((g - k) / kStages) & 1, nullptr);
+      if (nq > 0) (void)mbar_wait(q_full, (nq - 1) & 1, nullptr);
     }
+    __syncwarp();
   } else if (warp == 1) {
-    // ---------------------------------------------------------------- products
+    // ---------------------------------------------------------------- S = Q K^T
     if (lane == 0) {
-      constexpr uint32_t idesc_s = make_idesc_f16(128, 128, kBF16 ? 1 : 0, 0, 0);
-      constexpr uint32_t idesc_o = make_idesc_f16(128, D, kBF16 ? 1 : 0, 0, 1);
-      const uint64_t dQ = make_smem_desc(smem_u32(sQ), 16, 1024, 2);
-      const uint64_t dK = make_smem_desc(smem_u32(ring), 16, 1024, 2);
-      const uint64_t dV = make_smem_desc(smem_u32(ring), 16384, 1024, 2);
-      uint32_t pos = 0, seg = 0, np[2] = {0, 0};
+      constexpr uint32_t idesc = make_idesc_f16(128, 128, kBF16 ? 1 : 0, 0, 0);
+      const uint64_t dq = make_smem_desc(smem_u32(sQ), 16, 1024, 2);
+      const uint64_t dK = make_smem_desc(smem_u32(sK), 16, 1024, 2);
+      uint32_t g = 0, seg = 0;
       bool ok = true;
-      for (; w.left > 0 && ok; walk_next<kRows>(p, w), ++seg) {
-        const int T = min(w.left, w.tiles - w.at);
-        const int rows = min(kRows, p.G * p.T - w.grp * kRows);
-        const int n0 = kDual ? T : (T + 1) / 2, n1 = kDual ? (rows > 128 ? T : 0) : T / 2;
-        const int last = kDual ? (n1 > 0 ? 1 : 0) : 0;  // the stream after which a shared tile is free
-        ok = mbar_wait(q_full, seg & 1, abort_flag);
-        if (!ok) break;
-        tc_fence_after_sync();
-        auto scores = [&](int s, int g) {
-          const uint32_t at = pos + place_k<kDual>(g), st = at % kStages;
-          if (!mbar_wait(&kv_full[st], (at / kStages) & 1, abort_flag)) { ok = false; return; }
+      for (; w.left > 0 && ok; walk_next(p, sh, w)) {
+        const int T = own_tiles(p, sh, w, w.set * sh.wide + side);
+        if (T == 0) continue;
+        if (!mbar_wait(q_full, seg & 1, abort_flag)) break;
+        ++seg;
+        for (int i = 0; i < T; ++i, ++g) {
+          const uint32_t st = g % kStages, buf = g % kBufs;
+          if (!mbar_wait(&k_full[st], (g / kStages) & 1, abort_flag) ||
+              !mbar_wait(&buf_free[buf], ((g / kBufs) & 1) ^ 1, abort_flag)) {
+            ok = false;
+            break;
+          }
           tc_fence_after_sync();
-          const uint64_t dq = dQ + static_cast<uint64_t>((kDual ? s * C::kTile : 0) >> 4);
           const uint64_t dk = dK + static_cast<uint64_t>((st * C::kTile) >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint64_t o = (kk >> 2) * (16384 >> 4) + (kk & 3) * (32 >> 4);
-            mma_f16_ss(tmem + s * 128, dq + o, dk + o, idesc_s, kk > 0 ? 1u : 0u);
+            mma_f16_ss(tmem + buf * 128, dq + o, dk + o, idesc, kk > 0 ? 1u : 0u);
           }
-          if (!kDual || s == last) mma_commit(&kv_empty[st]);
-        };
-        scores(0, 0);
-        if (ok) mma_commit(&s_full[0]);
-        if (ok && n1 > 0) {
-          scores(1, kDual ? 0 : 1);
-          if (ok) mma_commit(&s_full[1]);
+          if constexpr (!C::kOneSignal) mma_commit(&k_empty[st]);
+          mma_commit(&s_full[buf]);
         }
-        for (int i = 0; i < n0 && ok; ++i) {
-          for (int s = 0; s < 2 && ok; ++s) {
-            const int ns = s ? n1 : n0;
-            if (i >= ns) continue;
-            const int g = kDual ? i : 2 * i + s;
-            const uint32_t at = pos + place_v<kDual>(g, T), st = at % kStages;
-            if (!mbar_wait(&kv_full[st], (at / kStages) & 1, abort_flag) ||
-                !mbar_wait(&p_full[s], np[s] & 1, abort_flag)) { ok = false; break; }
-            ++np[s];
-            tc_fence_after_sync();
-            const uint64_t dv = dV + static_cast<uint64_t>((st * C::kTile) >> 4);
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              mma_f16_ts(tmem + kTmemO + s * 128, tmem + s * 128 + kk * 8, dv + static_cast<uint64_t>(kk * (2048 >> 4)), idesc_o,
-                         (i > 0 || kk > 0) ? 1u : 0u);
-            if (!kDual || s == last) mma_commit(&kv_empty[st]);
-            if (i + 1 < ns) scores(s, kDual ? i + 1 : g + 2);
-            if (ok) mma_commit(&s_full[s]);  // S(i + 1), or the stream's finished O
-          }
-        }
-        pos += 2 * T;
       }
-      mma_commit(drain);
-      (void)mbar_wait(drain, 0, nullptr);
+      mma_commit(&drain[0]);
+      (void)mbar_wait(&drain[0], 0, nullptr);
     }
     __syncwarp();
-  } else if (warp >= 4) {
+  } else if (warp == 2) {
+    // ---------------------------------------------------------------- O += P V
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc_f16(128, D, kBF16 ? 1 : 0, 0, 1);
+      const uint64_t dV = make_smem_desc(smem_u32(sV), 16384, 1024, 2);
+      uint32_t g = 0;
+      bool ok = true;
+      for (; w.left > 0 && ok; walk_next(p, sh, w)) {
+        const int T = own_tiles(p, sh, w, w.set * sh.wide + side);
+        for (int i = 0; i < T; ++i, ++g) {
+          const uint32_t st = g % kStages, buf = g % kBufs;
+          // V normally lands early; P(g) is the event waited on last. All warps have read the
+          // previous segment's O before they release its first P.
+          if (!mbar_wait(&v_full[st], (g / kStages) & 1, abort_flag) ||
+              !mbar_wait(&p_full[buf], (g / kBufs) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint64_t dv = dV + static_cast<uint64_t>((st * C::kTile) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            mma_f16_ts(tmem + kTmemO, tmem + buf * 128 + (kk >> 2) * 64 + (kk & 3) * 8,
+                       dv + static_cast<uint64_t>(kk * (2048 >> 4)), idesc, (i > 0 || kk > 0) ? 1u : 0u);
+          if constexpr (!C::kOneSignal) mma_commit(&v_empty[st]);
+          mma_commit(&buf_free[buf]);
+        }
+      }
+      mma_commit(&drain[1]);
+      (void)mbar_wait(&drain[1], 0, nullptr);
+    }
+    __syncwarp();
+  } else {
     // ---------------------------------------------------------------- softmax and epilogue
-    const int s = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, st_tid = threadIdx.x - 128;
+    // Warp w owns TMEM lanes 32 * (w & 3) .. + 31 (rows) and key half kb = (w - 4) / 4 of every tile.
+    // A wait that gave up does not end the loops: the barriers stay matched, and every later wait
+    // returns at once.
+    const int quad = warp & 3, kb = (warp - 4) >> 2, r = quad * 32 + lane, tid = threadIdx.x - 128;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t t_s = tmem + lanes + s * 128, t_o = tmem + lanes + kTmemO + s * 128;
-    uint32_t pos = 0, ns_done = 0;
-    bool first = true;
-    for (; w.left > 0; walk_next<kRows>(p, w)) {
-      const int T = min(w.left, w.tiles - w.at);
+    const uint32_t t_o = tmem + lanes + kTmemO + kb * (D / 2);
+    uint32_t g = 0, xc = 0;
+    int seg = 0;
+    for (; w.left > 0; walk_next(p, sh, w)) {
+      const int grp = w.set * sh.wide + side;
+      const int T = own_tiles(p, sh, w, grp);
+      if (T == 0) continue;
+      ++seg;
       const Seq q = w.s;
-      const int R = p.G * p.T, row0 = w.grp * kRows;
-      const int rows = min(kRows, R - row0);
-      const int n0 = kDual ? T : (T + 1) / 2, n1 = kDual ? (rows > 128 ? T : 0) : T / 2;
-      const int count = s ? n1 : n0;
-      const int rr = kDual ? s * 128 + r : r;
-      const int t = (row0 + rr) / p.G;
-      const bool live = rr < rows && t < q.m;
+      const int t = grp * sh.nodes + r / p.G, rows = min(sh.nodes, p.T - grp * sh.nodes) * p.G;
+      const bool live = r < rows && t < q.m;
       const bool any_live = __any_sync(0xffffffffu, live);
-      const int key_lo = w.at * 128, keys = unit_keys<kRows>(p, q, w.grp);
-
-      // both streams have left the previous segment (its products are complete, its O is read)
-      if (!first) streams_sync();
-      first = false;
-      if (st_tid == 0) *odd_flag = 0;
-      for (int e = st_tid; e < kRows * (D / 8); e += 256) {
-        const int x = e / (D / 8), c = e - x * (D / 8);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (x < rows) {
-          const int row = row0 + x;
-          v = *reinterpret_cast<const uint4*>(static_cast<const InT*>(p.q) + w.b * p.qs[0] +
-                                              (w.hk * p.G + row % p.G) * p.qs[1] + (row / p.G) * p.qs[2] + c * 8);
-        }
-        *reinterpret_cast<uint4*>(sQ + (x >> 7) * C::kTile + (c >> 3) * 16384 + sw128_offset(x & 127, c & 7)) = v;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-      bool bad = false;
-      {
-        const int S = static_cast<int>(p.page_size), j1 = (min(keys, key_lo + T * 128) + S - 1) / S;
-        for (int j = key_lo / S + st_tid; j < j1; j += 256) {
-          const int pg = p.table[q.row * p.table_stride + j];
-          bad |= pg < 0 || pg >= p.pages;
-        }
-      }
-      bad = streams_sync_or(bad);
+      const int key_lo = w.at * 128, keys = group_keys(p, sh, q, grp, grp);
+      const bool has_tail = key_lo + T * 128 > q.ctx;
+      // the page of this lane's part of the warp's half tile, read one tile ahead: whether it is there
+      const int S = static_cast<int>(p.page_size), held = (q.len + S - 1) / S;
+      auto lost_page = [&](int i) -> bool {
+        const int j = (key_lo + i * 128 + kb * 64) / S + lane;
+        if (lane * S >= 64 || i >= T || j >= held) return false;
+        const int pg = p.table[q.row * p.table_stride + j];
+        return pg < 0 || pg >= p.pages;
+      };
+      bool lost = lost_page(0);
 
       float m_run = -INFINITY, l = 0.f;
-      for (int i = 0; i < count; ++i) {
-        const int g = kDual ? i : 2 * i + s;
-        const int key0 = key_lo + g * 128;
-        const bool tail = bad || key0 + 128 > q.ctx;
-        (void)mbar_wait(&s_full[s], ns_done & 1, abort_flag);
-        ++ns_done;
+      for (int i = 0; i < T; ++i, ++g) {
+        const uint32_t buf = g % kBufs;
+        const int key0 = key_lo + i * 128;
+        const bool bad = __any_sync(0xffffffffu, lost), tail = bad || key0 + 128 > q.ctx;
+        lost = lost_page(i + 1);
+        const uint32_t t_s = tmem + lanes + buf * 128 + kb * 64;  // S in, P out
+        (void)mbar_wait(&s_full[buf], (g / kBufs) & 1, abort_flag);
         tc_fence_after_sync();
-        if (tail && (!kDual || s == 0)) {
-          const uint32_t at = pos + place_v<kDual>(g, T), sg = at % kStages;
-          (void)mbar_wait(&kv_full[sg], (at / kStages) & 1, abort_flag);
-          const int key = key0 + r;
-          if (key >= q.ctx) {
-            if (clean_v_row<D, kBF16>(ring + sg * C::kTile, r, key, q)) *reinterpret_cast<volatile int*>(odd_flag) = 1;
+        uint64_t see = ~0ull;
+        if (tail) {
+          // S(g) came after PV(g - 3), so V(g)'s barrier is at most this phase behind; P(g) is not
+          // released before V(g) is clean, and PV(g) frees V(g)
+          (void)mbar_wait(&v_full[g % kStages], (g / kStages) & 1, abort_flag);
+          if (key0 + r >= q.ctx) {
+            if (clean_v_row<D, kBF16>(sV + (g % kStages) * C::kTile, r, kb, key0 + r, q)) *reinterpret_cast<volatile int*>(odd_seg) = seg;
             fence_proxy_async_smem();
           }
+          see = live ? seen_bits(p, q, w.b, t, key0 + kb * 64, bad) : 0ull;
         }
         if (any_live) {
-          Bits see{~0ull, ~0ull};
-          if (tail) see = live ? seen_bits(p, q, w.b, t, key0, bad) : Bits{0, 0};
-          float mx = -INFINITY;
+          uint32_t s[64];
+          tmem_ld32(t_s, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+          tmem_ld32(t_s + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+          tmem_wait_ld();
+          float m8[8];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t x[32];
-            tmem_ld32(t_s + 32 * c, x);
-            tmem_wait_ld();
-            if (tail) {
-              const uint32_t word = static_cast<uint32_t>((c < 2 ? see.lo : see.hi) >> (32 * (c & 1)));
+          for (int u = 0; u < 8; ++u) m8[u] = -INFINITY;
+          if (tail) {
 #pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (word >> k & 1u) mx = fmaxf(mx, __uint_as_float(x[k]));
-            } else {
-              float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+            for (int c = 0; c < 64; ++c)
+              if (see >> c & 1ull) m8[c & 7] = fmaxf(m8[c & 7], __uint_as_float(s[c]));
+          } else {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(x[k]));
-              mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-            }
+            for (int c = 0; c < 64; c += 2)
+              m8[(c >> 1) & 7] = fmax3(m8[(c >> 1) & 7], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
           }
-          const float m_tile = mx * p.scale_log2;
+          const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
+          // two buffers by parity: one is rewritten after the exchange in between
+          float* xs = xchg + (xc & 1u) * 256;
+          xs[kb * 128 + r] = mx;
+          pair_sync(quad);
+          ++xc;
+          const float m_tile = fmaxf(mx, xs[(kb ^ 1) * 128 + r]) * p.scale_log2;
           float alpha = 1.f;
           if (m_run == -INFINITY) {
             m_run = m_tile;
@@ -811,9 +868,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             m_run = m_tile;
             l *= alpha;
           }
+          const float sub = m_run == -INFINITY ? 0.f : m_run;  // nothing above -inf so far: weights 0
+          l += tail ? weights<kBF16, true>(s, see, p.scale_log2, sub, t_s) : weights<kBF16, false>(s, see, p.scale_log2, sub, t_s);
           if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
+            // PV(g - 1) has completed: its barrier's phase before, PV(g - 4), was needed by S(g - 1)
+            (void)mbar_wait(&buf_free[(g - 1) % kBufs], ((g - 1) / kBufs) & 1, abort_flag);
+            tc_fence_after_sync();
+#pragma unroll
+            for (int c = 0; c < D / 2; c += 32) {
               uint32_t x[32];
               tmem_ld32(t_o + c, x);
               tmem_wait_ld();
@@ -822,134 +884,83 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tmem_st32(t_o + c, x);
             }
           }
-          const float sub = m_run == -INFINITY ? 0.f : m_run;  // all scores -inf so far: weights 0
-          float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t x[32], y[16];
-            tmem_ld32(t_s + 32 * c, x);
-            tmem_wait_ld();
-            const uint32_t word = static_cast<uint32_t>((c < 2 ? see.lo : see.hi) >> (32 * (c & 1)));
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              float p0 = ex2(fmaf(__uint_as_float(x[k]), p.scale_log2, -sub));
-              float p1 = ex2(fmaf(__uint_as_float(x[k + 1]), p.scale_log2, -sub));
-              if (tail) {
-                p0 = word >> k & 1u ? p0 : 0.f;
-                p1 = word >> (k + 1) & 1u ? p1 : 0.f;
-              }
-              l4[(k >> 1) & 3] += p0 + p1;
-              y[k >> 1] = pack2<kBF16>(p0, p1);
-            }
-            tmem_st16(t_s + 16 * c, y);
-          }
-          l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
           tmem_wait_st();
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[s]);
+        if (lane == 0) mbar_arrive(&p_full[buf]);
       }
-      if (count > 0) {
-        (void)mbar_wait(&s_full[s], ns_done & 1, abort_flag);
-        ++ns_done;
-        tc_fence_after_sync();
-      }
-      pos += 2 * T;
 
-      // epilogue: dual: this stream's rows; single: half the columns of the row's two sums
-      float m_other = -INFINITY, l_other = 0.f;
-      tc_fence_before_sync();
-      if constexpr (!kDual) {
-        streams_sync();  // all products are complete: Q's memory is free, both O can be read
-        float2* xchg = reinterpret_cast<float2*>(sQ);
-        xchg[s * 128 + r] = make_float2(m_run, l);
-        streams_sync();
-        const float2 o = xchg[(s ^ 1) * 128 + r];
-        m_other = o.x;
-        l_other = o.y;
-      } else {
-        streams_sync();
-      }
+      // epilogue: the row's two threads take half the columns each
+      (void)mbar_wait(&buf_free[(g - 1) % kBufs], ((g - 1) / kBufs) & 1, abort_flag);
       tc_fence_after_sync();
-      const bool odd = *reinterpret_cast<volatile int*>(odd_flag) != 0;
-      if (any_live || (kDual ? s * 128 + quad * 32 : quad * 32) < rows) {
-        const float m_all = fmaxf(m_run, m_other);
-        const float m_ref = m_all == -INFINITY ? 0.f : m_all;
-        const float w_own = ex2(m_run - m_ref), w_other = ex2(m_other - m_ref);  // 2^-inf = 0
-        const float l_all = l * w_own + l_other * w_other;
-        const bool whole = T == w.tiles;
-        const bool own_used = count > 0 && any_live, other_used = !kDual && (s ? n0 : n1) > 0 && any_live;
-        const float inv = l_all != 0.f ? 1.f / l_all : 0.f;
-        const int row = row0 + rr;
-        InT* orow = static_cast<InT*>(p.out) + w.b * p.os[0] + (w.hk * p.G + row % p.G) * p.os[1] + t * p.os[2];
-        const int slot = 2 * static_cast<int>(blockIdx.x) + (w.left == s_begin[2] ? 0 : 1);
-        const int64_t prow = static_cast<int64_t>(slot) * p.part_rows + rr;
-        constexpr int kCols = kDual ? D : D / 2;
-        const int col0 = kDual ? 0 : s * kCols;
-#pragma unroll 1
-        for (int c = col0; c < col0 + kCols; c += 32) {
-          float o[32];
+      if (any_live) {
+        float* xs = xchg + (xc & 1u) * 256;
+        xs[kb * 128 + r] = l;
+        pair_sync(quad);
+        ++xc;
+        l += xs[(kb ^ 1) * 128 + r];
+      }
+      if (has_tail) softmax_sync();  // all warps have cleaned their part of V
+      if (quad * 32 < rows) {
+        const bool odd = has_tail && *reinterpret_cast<volatile int*>(odd_seg) == seg;
+        const bool whole = T == tiles_of(keys);
+        const float inv = live && l != 0.f ? 1.f / l : 0.f;
+        const int h = w.hk * p.G + r % p.G;
+        InT* orow = static_cast<InT*>(p.out) + w.b * p.os[0] + h * p.os[1] + t * p.os[2] + kb * (D / 2);
+        const int slot = 2 * static_cast<int>(blockIdx.x) + (w.left == begin[2] ? 0 : 1);
+        const int64_t prow = static_cast<int64_t>(slot) * p.part_rows + r;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0.f;
-          if (own_used) {
-            uint32_t x[32];
+        for (int c = 0; c < D / 2; c += 32) {
+          uint32_t x[32];
+          if (any_live) {
             tmem_ld32(t_o + c, x);
             tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(x[k]) * w_own;
           }
-          if (other_used) {
-            uint32_t x[32];
-            tmem_ld32(tmem + lanes + kTmemO + (s ^ 1) * 128 + c, x);
-            tmem_wait_ld();
+          if (r >= rows) continue;
+          if (odd && live) {
+            float more[32];  // rare: kept out of the sum's registers
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = fmaf(__uint_as_float(x[k]), w_other, o[k]);
+            for (int k = 0; k < 32; ++k) more[k] = 0.f;
+            fix_up<InT>(p, q, w.b, w.hk, t, key_lo, key_lo + T * 128, kb * (D / 2) + c, more);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) + more[k]);
           }
-          if (rr < rows) {
-            if (odd && live) {
-              float more[32];  // rare: kept out of the sum's registers
+          if (!live) {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) more[k] = 0.f;
-              fix_up<InT>(p, q, w.b, w.hk, t, key_lo, key_lo + T * 128, c, more);
+            for (int k = 0; k < 32; ++k) x[k] = 0u;
+          }
+          if (whole) {
+            if (p.out_vec) {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] += more[k];
-            }
-            if (whole) {
-              const float f = live ? inv : 0.f;
-              if (p.out_vec) {
+              for (int k = 0; k < 32; k += 8) {
+                uint32_t y[4];
 #pragma unroll
-                for (int k = 0; k < 32; k += 8) {
-                  uint4 v;
-                  v.x = live ? pack2<kBF16>(o[k] * f, o[k + 1] * f) : 0u;
-                  v.y = live ? pack2<kBF16>(o[k + 2] * f, o[k + 3] * f) : 0u;
-                  v.z = live ? pack2<kBF16>(o[k + 4] * f, o[k + 5] * f) : 0u;
-                  v.w = live ? pack2<kBF16>(o[k + 6] * f, o[k + 7] * f) : 0u;
-                  *reinterpret_cast<uint4*>(orow + c + k) = v;
-                }
-              } else {
-#pragma unroll
-                for (int k = 0; k < 32; ++k) orow[c + k] = from_f32<InT>(live ? o[k] * f : 0.f);
+                for (int u = 0; u < 4; ++u)
+                  y[u] = pack2<kBF16>(__uint_as_float(x[k + 2 * u]) * inv, __uint_as_float(x[k + 2 * u + 1]) * inv);
+                *reinterpret_cast<uint4*>(orow + c + k) = make_uint4(y[0], y[1], y[2], y[3]);
               }
             } else {
-              float4* po = reinterpret_cast<float4*>(p.part_o + prow * D + c);
 #pragma unroll
-              for (int k = 0; k < 8; ++k) po[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+              for (int k = 0; k < 32; ++k) orow[c + k] = from_f32<InT>(__uint_as_float(x[k]) * inv);
             }
-          }
-        }
-        if (rr < rows && (kDual || s == 0)) {
-          if (whole) {
-            if (p.lse)
-              p.lse[(static_cast<int64_t>(w.b) * p.Hq + w.hk * p.G + row % p.G) * p.T + t] =
-                  live ? (m_ref + log2f(l_all)) * kLn2 : -INFINITY;
           } else {
-            p.part_ml[prow * 2] = live ? m_all : -INFINITY;
-            p.part_ml[prow * 2 + 1] = live ? l_all : 0.f;
+            uint4* po = reinterpret_cast<uint4*>(p.part_o + prow * D + kb * (D / 2) + c);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) po[k] = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
           }
         }
-        tc_fence_before_sync();
+        if (r < rows && kb == 0) {
+          if (whole) {
+            const float m_ref = m_run == -INFINITY ? 0.f : m_run;
+            if (p.lse) p.lse[(static_cast<int64_t>(w.b) * p.Hq + h) * p.T + t] = live ? (m_ref + log2f(l)) * kLn2 : -INFINITY;
+          } else {
+            p.part_ml[prow * 2] = live ? m_run : -INFINITY;
+            p.part_ml[prow * 2 + 1] = live ? l : 0.f;
+          }
+        }
       }
+      tc_fence_before_sync();
     }
   }
   __syncthreads();
@@ -958,19 +969,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // Adds a cut unit's partial sums: one warp per row, in key order.
-template <int D, bool kBF16, bool kDual>
-__global__ void __launch_bounds__(256) join_kernel(const Params p, int ctas_max) {
-  using C = Cfg<D, kDual>;
+template <int D, bool kBF16>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params p, int ctas_max) {
   using InT = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
-  constexpr int kRows = C::kRows;
   __shared__ int s_c0, s_c1, s_first;
-  const int groups = (p.G * p.T + kRows - 1) / kRows;
+  const Share sh = share_of(p.G, p.T);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int grp = blockIdx.x % groups, hk = blockIdx.x / groups % p.Hkv, b = blockIdx.x / groups / p.Hkv;
+  const int grp = blockIdx.x % sh.groups, hk = blockIdx.x / sh.groups % p.Hkv, b = blockIdx.x / sh.groups / p.Hkv;
+  const int set = grp / sh.wide, side = grp % sh.wide;
   if (warp == 0) {
     int64_t total = 0, before = 0;
     for (int i = lane; i < p.n; i += 32) {
-      const int64_t x = static_cast<int64_t>(seq_tiles<kRows>(p, load_seq(p, i))) * p.Hkv;
+      const int64_t x = static_cast<int64_t>(head_weight(p, sh, load_seq(p, i))) * p.Hkv;
       total += x;
       if (i < b) before += x;
     }
@@ -980,33 +990,33 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, int ctas_max)
       before += __shfl_xor_sync(0xffffffffu, before, o);
     }
     const Seq s = load_seq(p, b);
-    before += static_cast<int64_t>(hk) * seq_tiles<kRows>(p, s);
-    for (int g = 0; g < grp; ++g) before += unit_tiles<kRows>(p, s, g);
-    const int64_t end = before + unit_tiles<kRows>(p, s, grp);
-    const int64_t ctas = range_ctas(total, ctas_max, p.least);
-    // the CTA of flat tile f is the largest c with total * c / ctas <= f
-    int64_t c0 = (before * ctas + ctas - 1) / total, c1 = ((end - 1) * ctas + ctas - 1) / total;
-    while (range_start(total, ctas, c0) > before) --c0;
-    while (c0 + 1 < ctas && range_start(total, ctas, c0 + 1) <= before) ++c0;
-    while (range_start(total, ctas, c1) > end - 1) --c1;
-    while (c1 + 1 < ctas && range_start(total, ctas, c1 + 1) <= end - 1) ++c1;
+    before += static_cast<int64_t>(hk) * head_weight(p, sh, s);
+    for (int g = 0; g < set; ++g) before += unit_tiles(p, sh, s, g);
+    const int64_t end = before + tiles_of(group_keys(p, sh, s, grp, grp));
+    const int64_t ranges = range_count(total, ctas_max / sh.wide, p.least);
+    // the range of flat tile f is the largest c with total * c / ranges <= f
+    int64_t c0 = (before * ranges + ranges - 1) / total, c1 = ((end - 1) * ranges + ranges - 1) / total;
+    while (range_start(total, ranges, c0) > before) --c0;
+    while (c0 + 1 < ranges && range_start(total, ranges, c0 + 1) <= before) ++c0;
+    while (range_start(total, ranges, c1) > end - 1) --c1;
+    while (c1 + 1 < ranges && range_start(total, ranges, c1 + 1) <= end - 1) ++c1;
     if (lane == 0) {
       s_c0 = static_cast<int>(c0);
       s_c1 = static_cast<int>(c1);
-      s_first = range_start(total, ctas, c0) >= before;  // the unit begins CTA c0's range
+      s_first = range_start(total, ranges, c0) >= before;  // the unit begins range c0
     }
   }
   __syncthreads();
   const int c0 = s_c0, c1 = s_c1;
   if (c0 == c1) return;
-  const int rr = blockIdx.y * 8 + warp, row = grp * kRows + rr;
+  const int rr = blockIdx.y * 8 + warp, t = grp * sh.nodes + rr / p.G;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (rr >= kRows || row >= p.G * p.T) return;
+  if (rr >= sh.nodes * p.G || t >= p.T) return;
+  auto part = [&](int c) -> int64_t {  // the row's place in range c's partial slot
+    return (2 * (static_cast<int64_t>(c) * sh.wide + side) + (c == c0 && !s_first ? 1 : 0)) * p.part_rows + rr;
+  };
   float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) {
-    const int slot = 2 * c + (c == c0 && !s_first ? 1 : 0);
-    m = fmaxf(m, p.part_ml[(static_cast<int64_t>(slot) * p.part_rows + rr) * 2]);
-  }
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.part_ml[part(c) * 2]);
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float m_ref = m == -INFINITY ? 0.f : m;
@@ -1016,14 +1026,13 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, int ctas_max)
   for (int k = 0; k < kV; ++k) acc[k] = 0.f;
 #pragma unroll 4
   for (int c = c0; c <= c1; ++c) {
-    const int slot = 2 * c + (c == c0 && !s_first ? 1 : 0);
-    const int64_t x = static_cast<int64_t>(slot) * p.part_rows + rr;
+    const int64_t x = part(c);
     const float wgt = ex2(p.part_ml[x * 2] - m_ref);
     l = fmaf(wgt, p.part_ml[x * 2 + 1], l);
 #pragma unroll
     for (int k = 0; k < kV; ++k) acc[k] = fmaf(wgt, p.part_o[x * D + lane * kV + k], acc[k]);
   }
-  const int h = hk * p.G + row % p.G, t = row / p.G;
+  const int h = hk * p.G + rr % p.G;
   InT* o = static_cast<InT*>(p.out) + b * p.os[0] + h * p.os[1] + t * p.os[2] + lane * kV;
   const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
@@ -1038,15 +1047,15 @@ inline int simt_splits(int64_t units, int64_t tokens) {
 }
 
 struct Layout {
-  bool tc, dual;
+  bool tc, whole;
   int splits, part_rows, ctas;
   int64_t units;
   size_t part_o, part_ml, total;
 };
 
-inline bool use_tensor_cores(const cab_page_cache* c) {
+inline bool use_tensor_cores(const cab_page_cache* c, int64_t G) {
   if (c->dtype != CAB_DTYPE_BF16 && c->dtype != CAB_DTYPE_F16) return false;
-  if (c->dim != 64 && c->dim != 128) return false;
+  if ((c->dim != 64 && c->dim != 128) || G > 128) return false;
   const int64_t S = c->page_size;
   if (!(S == 8 || S == 16 || S == 32 || S == 64 || S % 128 == 0)) return false;
   if (!aligned16(c->k_pages) || !aligned16(c->v_pages)) return false;
@@ -1058,15 +1067,15 @@ inline bool use_tensor_cores(const cab_page_cache* c) {
 
 inline Layout layout(const cab_page_cache* c, int64_t n, int64_t Hq, int64_t T) {
   Layout L{};
-  const int64_t R = Hq / c->heads * T, D = c->dim;
-  L.tc = use_tensor_cores(c);
+  const int64_t G = Hq / c->heads, R = G * T, D = c->dim;
+  L.tc = use_tensor_cores(c, G);
   if (L.tc) {
-    // More than 128 rows a KV head: both halves of a 256-row group use each K / V tile.
-    L.dual = R > 128;
-    const int64_t rows = L.dual ? 256 : 128;
-    L.units = n * c->heads * ((R + rows - 1) / rows);
-    L.part_rows = static_cast<int>(std::min(R, rows));
+    const Share sh = share_of(static_cast<int>(G), static_cast<int>(T));
+    L.units = n * c->heads * sh.groups;
+    L.part_rows = static_cast<int>(G * std::min<int64_t>(T, sh.nodes));
+    L.whole = c->width * c->page_size <= kWholeTiles * 128;
     L.ctas = current_sm_count();
+    if (L.whole) return L;
     const size_t slots = static_cast<size_t>(L.ctas) * 2 * L.part_rows;
     L.part_ml = slots * D * 4;
     L.total = L.part_ml + slots * 8;
@@ -1090,12 +1099,24 @@ inline int page_map(CUtensorMap* map, const void* base, const cab_page_cache* c,
   return make_tensor_map(map, tma_type(static_cast<int>(c->dtype)), 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int D, bool kBF16, bool kDual>
-int launch_tc(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, const Layout& L, cudaStream_t st) {
-  using C = Cfg<D, kDual>;
-  cudaFuncSetAttribute(tc_kernel<D, kBF16, kDual>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-  tc_kernel<D, kBF16, kDual><<<L.ctas, kTcThreads, C::kSmem, st>>>(km, vm, p);
+// The query as [n, Hkv, T, G, D]: a box is the G rows of a group's nodes (64 columns of them).
+inline int query_map(CUtensorMap* map, const void* q, const Params& p, int64_t dtype) {
+  const uint64_t dims[5] = {static_cast<uint64_t>(p.D), static_cast<uint64_t>(p.G), static_cast<uint64_t>(p.T),
+                            static_cast<uint64_t>(p.Hkv), static_cast<uint64_t>(p.n)};
+  const uint64_t strides[4] = {static_cast<uint64_t>(p.qs[1]) * 2, static_cast<uint64_t>(p.qs[2]) * 2,
+                               static_cast<uint64_t>(p.qs[1]) * 2 * p.G, static_cast<uint64_t>(p.qs[0]) * 2};
+  const uint32_t box[5] = {64, static_cast<uint32_t>(p.G), static_cast<uint32_t>(std::min(p.T, 128 / p.G)), 1, 1};
+  return make_tensor_map(map, tma_type(static_cast<int>(dtype)), 5, q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int D, bool kBF16>
+int launch_tc(const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& qm, const Params& p, const Layout& L,
+              cudaStream_t st) {
+  using C = Cfg<D>;
+  cudaFuncSetAttribute(tc_kernel<D, kBF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  tc_kernel<D, kBF16><<<L.ctas, kTcThreads, C::kSmem, st>>>(km, vm, qm, p);
   if (int rc = check_launch("tree_attn tc_kernel")) return rc;
+  if (L.whole) return CAB_OK;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3(static_cast<unsigned>(L.units), static_cast<unsigned>((L.part_rows + 7) / 8));
@@ -1105,13 +1126,8 @@ int launch_tc(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, con
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, join_kernel<D, kBF16, kDual>, p, L.ctas);
+  cudaLaunchKernelEx(&cfg, join_kernel<D, kBF16>, p, L.ctas);
   return check_launch("tree_attn join_kernel");
-}
-
-template <int D, bool kBF16>
-int launch_tc_rows(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, const Layout& L, cudaStream_t st) {
-  return L.dual ? launch_tc<D, kBF16, true>(km, vm, p, L, st) : launch_tc<D, kBF16, false>(km, vm, p, L, st);
 }
 
 template <typename T, int DC>
@@ -1215,19 +1231,22 @@ extern "C" int cab_tree_attn_fwd(const cab_page_cache* cache, int64_t layer, con
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (L.tc) {
     if (!aligned16(q)) return fail(CAB_ERR_INVALID_ARG, "tree_attn: q must be 16-byte aligned");
-    p.least = 2;
+    p.least = L.whole ? 1 : 2;
+    p.whole_units = L.whole;
     p.part_rows = L.part_rows;
     p.out_vec = aligned16(out);
     for (int i = 0; i < 3; ++i) {
-      if (q_strides[i] % 8 != 0) return fail(CAB_ERR_INVALID_ARG, "tree_attn: q strides must be multiples of 16 bytes");
+      if (q_strides[i] <= 0 || q_strides[i] % 8 != 0)
+        return fail(CAB_ERR_INVALID_ARG, "tree_attn: q strides must be positive multiples of 16 bytes");
       p.out_vec = p.out_vec && o_strides[i] % 8 == 0;
     }
-    CUtensorMap km{}, vm{};
+    CUtensorMap km{}, vm{}, qm{};
+    if (int rc = query_map(&qm, q, p, cache->dtype)) return rc;
     if (int rc = page_map(&km, p.k, cache, cache->k_strides)) return rc;
     if (int rc = page_map(&vm, p.v, cache, cache->v_strides)) return rc;
     if (cache->dtype == CAB_DTYPE_BF16)
-      return cache->dim == 128 ? launch_tc_rows<128, true>(km, vm, p, L, st) : launch_tc_rows<64, true>(km, vm, p, L, st);
-    return cache->dim == 128 ? launch_tc_rows<128, false>(km, vm, p, L, st) : launch_tc_rows<64, false>(km, vm, p, L, st);
+      return cache->dim == 128 ? launch_tc<128, true>(km, vm, qm, p, L, st) : launch_tc<64, true>(km, vm, qm, p, L, st);
+    return cache->dim == 128 ? launch_tc<128, false>(km, vm, qm, p, L, st) : launch_tc<64, false>(km, vm, qm, p, L, st);
   }
   switch (cache->dtype) {
     case CAB_DTYPE_F32: return launch_simt_d<float>(p, L.units, st);
