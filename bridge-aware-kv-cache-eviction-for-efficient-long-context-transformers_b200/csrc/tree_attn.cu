@@ -18,7 +18,9 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <type_traits>
 
 namespace cab {
 namespace tree {
@@ -305,6 +307,7 @@ constexpr float kRescaleThreshold = 8.0f;
 constexpr int kBufs = 3;
 constexpr uint32_t kTmemO = 384;
 constexpr int kMaxShare = 4;
+constexpr int kWindow = 16;  // tiles whose page numbers the softmax warps check at a time
 constexpr int kWholeTiles = 4;  // rows of at most this many tiles are not cut: no join
 
 template <int D>
@@ -427,7 +430,7 @@ __device__ __forceinline__ Begin find_range(const Params& p, const Share& sh, in
 __device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
 // Which of the keys key0 .. key0 + 63 node t of sequence b sees.
-__device__ __noinline__ uint64_t seen_bits(const Params& p, const Seq& s, int b, int t, int key0, bool bad_pages) {
+__device__ __forceinline__ uint64_t seen_bits(const Params& p, const Seq& s, int b, int t, int key0, bool bad_pages) {
   const int c = s.ctx - key0;
   uint64_t w = low_bits(c);
   if (p.parents) {
@@ -459,7 +462,7 @@ __device__ __noinline__ uint64_t seen_bits(const Params& p, const Seq& s, int b,
 // Adds to 32 columns of a row's sum the values that are not finite of the nodes it sees among
 // keys [lo, hi): they were taken out of the product.
 template <typename T>
-__device__ __noinline__ void fix_up(const Params& p, const Seq& s, int b, int hk, int t, int lo, int hi, int col, float* o) {
+__device__ __forceinline__ void fix_up(const Params& p, const Seq& s, int b, int hk, int t, int lo, int hi, int col, float* o) {
   for (int key = max(lo, s.ctx); key < min(hi, s.len); ++key) {
     if (!sees(p, b, t, key - s.ctx)) continue;
     const int64_t pg = p.table[s.row * p.table_stride + key / p.page_size], slot = key % p.page_size;
@@ -790,10 +793,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // Warp w owns TMEM lanes 32 * (w & 3) .. + 31 (rows) and key half kb = (w - 4) / 4 of every tile.
     // A wait that gave up does not end the loops: the barriers stay matched, and every later wait
     // returns at once.
-    const int quad = warp & 3, kb = (warp - 4) >> 2, r = quad * 32 + lane, tid = threadIdx.x - 128;
+    const int quad = warp & 3, kb = (warp - 4) >> 2, r = quad * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t t_o = tmem + lanes + kTmemO + kb * (D / 2);
-    uint32_t g = 0, xc = 0;
+    // tile g's S / P buffer and barrier phase, and its V stage and phase, counted instead of divided
+    uint32_t buf = 0, phase = 0, stage = 0, vphase = 0, xc = 0;
     int seg = 0;
     for (; w.left > 0; walk_next(p, sh, w)) {
       const int grp = w.set * sh.wide + side;
@@ -806,32 +810,34 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const bool any_live = __any_sync(0xffffffffu, live);
       const int key_lo = w.at * 128, keys = group_keys(p, sh, q, grp, grp);
       const bool has_tail = key_lo + T * 128 > q.ctx;
-      // the page of this lane's part of the warp's half tile, read one tile ahead: whether it is there
       const int S = static_cast<int>(p.page_size), held = (q.len + S - 1) / S;
-      auto lost_page = [&](int i) -> bool {
-        const int j = (key_lo + i * 128 + kb * 64) / S + lane;
-        if (lane * S >= 64 || i >= T || j >= held) return false;
-        const int pg = p.table[q.row * p.table_stride + j];
-        return pg < 0 || pg >= p.pages;
+      // Whether a page of tiles i .. i + kWindow - 1 (this warp's 64 keys of each) is outside the pool.
+      auto lost_pages = [&](int i) -> bool {
+        const int k0 = key_lo + i * 128, j0 = k0 / S, j1 = min(held, (min(k0 + kWindow * 128, key_lo + T * 128) + S - 1) / S);
+        bool lost = false;
+        for (int j = j0 + lane; j < j1; j += 32) {
+          const int pg = p.table[q.row * p.table_stride + j];
+          lost |= pg < 0 || pg >= p.pages;
+        }
+        return __any_sync(0xffffffffu, lost);
       };
-      bool lost = lost_page(0);
 
       float m_run = -INFINITY, l = 0.f;
-      for (int i = 0; i < T; ++i, ++g) {
-        const uint32_t buf = g % kBufs;
-        const int key0 = key_lo + i * 128;
-        const bool bad = __any_sync(0xffffffffu, lost), tail = bad || key0 + 128 > q.ctx;
-        lost = lost_page(i + 1);
+      uint32_t before = 0, before_phase = 0;  // the previous tile's buffer
+      // One tile, kMasked: some of its keys are nodes, past the length or on a lost page.
+      auto tile = [&](auto masked, int i, bool bad) {
+        constexpr bool kMasked = decltype(masked)::value;
         const uint32_t t_s = tmem + lanes + buf * 128 + kb * 64;  // S in, P out
-        (void)mbar_wait(&s_full[buf], (g / kBufs) & 1, abort_flag);
+        (void)mbar_wait(&s_full[buf], phase, abort_flag);
         tc_fence_after_sync();
         uint64_t see = ~0ull;
-        if (tail) {
+        if constexpr (kMasked) {
           // S(g) came after PV(g - 3), so V(g)'s barrier is at most this phase behind; P(g) is not
           // released before V(g) is clean, and PV(g) frees V(g)
-          (void)mbar_wait(&v_full[g % kStages], (g / kStages) & 1, abort_flag);
+          const int key0 = key_lo + i * 128;
+          (void)mbar_wait(&v_full[stage], vphase, abort_flag);
           if (key0 + r >= q.ctx) {
-            if (clean_v_row<D, kBF16>(sV + (g % kStages) * C::kTile, r, kb, key0 + r, q)) *reinterpret_cast<volatile int*>(odd_seg) = seg;
+            if (clean_v_row<D, kBF16>(sV + stage * C::kTile, r, kb, key0 + r, q)) *reinterpret_cast<volatile int*>(odd_seg) = seg;
             fence_proxy_async_smem();
           }
           see = live ? seen_bits(p, q, w.b, t, key0 + kb * 64, bad) : 0ull;
@@ -844,10 +850,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           float m8[8];
 #pragma unroll
           for (int u = 0; u < 8; ++u) m8[u] = -INFINITY;
-          if (tail) {
+          if constexpr (kMasked) {
+            const uint32_t lo = static_cast<uint32_t>(see), hi = static_cast<uint32_t>(see >> 32);
 #pragma unroll
             for (int c = 0; c < 64; ++c)
-              if (see >> c & 1ull) m8[c & 7] = fmaxf(m8[c & 7], __uint_as_float(s[c]));
+              if ((c < 32 ? lo : hi) >> (c & 31) & 1u) m8[c & 7] = fmaxf(m8[c & 7], __uint_as_float(s[c]));
           } else {
 #pragma unroll
             for (int c = 0; c < 64; c += 2)
@@ -869,10 +876,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             l *= alpha;
           }
           const float sub = m_run == -INFINITY ? 0.f : m_run;  // nothing above -inf so far: weights 0
-          l += tail ? weights<kBF16, true>(s, see, p.scale_log2, sub, t_s) : weights<kBF16, false>(s, see, p.scale_log2, sub, t_s);
+          l += weights<kBF16, kMasked>(s, see, p.scale_log2, sub, t_s);
           if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
             // PV(g - 1) has completed: its barrier's phase before, PV(g - 4), was needed by S(g - 1)
-            (void)mbar_wait(&buf_free[(g - 1) % kBufs], ((g - 1) / kBufs) & 1, abort_flag);
+            (void)mbar_wait(&buf_free[before], before_phase, abort_flag);
             tc_fence_after_sync();
 #pragma unroll
             for (int c = 0; c < D / 2; c += 32) {
@@ -889,10 +896,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[buf]);
+        before = buf;
+        before_phase = phase;
+        if (++buf == kBufs) {
+          buf = 0;
+          phase ^= 1u;
+        }
+        if (++stage == kStages) {
+          stage = 0;
+          vphase ^= 1u;
+        }
+      };
+      const int plain = max(0, min(T, (q.ctx - key_lo) / 128));  // tiles of context alone
+      for (int i0 = 0; i0 < T; i0 += kWindow) {
+        const bool bad = lost_pages(i0);
+        const int i1 = min(T, i0 + kWindow), im = bad ? i0 : min(i1, max(i0, plain));
+        for (int i = i0; i < im; ++i) tile(std::false_type{}, i, false);
+        for (int i = im; i < i1; ++i) tile(std::true_type{}, i, bad);
       }
 
       // epilogue: the row's two threads take half the columns each
-      (void)mbar_wait(&buf_free[(g - 1) % kBufs], ((g - 1) / kBufs) & 1, abort_flag);
+      (void)mbar_wait(&buf_free[before], before_phase, abort_flag);
       tc_fence_after_sync();
       if (any_live) {
         float* xs = xchg + (xc & 1u) * 256;
@@ -1113,7 +1137,13 @@ template <int D, bool kBF16>
 int launch_tc(const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& qm, const Params& p, const Layout& L,
               cudaStream_t st) {
   using C = Cfg<D>;
-  cudaFuncSetAttribute(tc_kernel<D, kBF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  static std::atomic<uint64_t> ready{0};  // devices on which the kernel has been set up
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1u)) {
+    cudaFuncSetAttribute(tc_kernel<D, kBF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (dev >= 0 && dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   tc_kernel<D, kBF16><<<L.ctas, kTcThreads, C::kSmem, st>>>(km, vm, qm, p);
   if (int rc = check_launch("tree_attn tc_kernel")) return rc;
   if (L.whole) return CAB_OK;
