@@ -135,6 +135,11 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def raw_stream(index: int) -> int:
+    """The current stream's handle on device ``index``, without building a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def strides3(t: torch.Tensor):
     """{b, h, n} element strides of a [B,H,N,D] tensor whose last dimension is dense."""
     if t.stride(3) != 1:

@@ -26,7 +26,7 @@ from typing import Optional, Union
 import torch
 
 from .. import _lib
-from ..kernels.tree_attention import attend_cache, describe_cache, int32_vector, on_device
+from ..kernels.tree_attention import attend_cache, call_on, describe_cache, int32_vector
 
 STATUS = {1: "not enough free pages", 2: "a row would hold more tokens than its table row has pages for",
           4: "a row outside the table, or named twice as a destination",
@@ -76,23 +76,19 @@ class PagedKVCache:
         else:
             grow_value, grow = int(grow), None
         L = _lib.lib()
-        with on_device(self.device):
-            size = self._sizes.get(n)
-            if size is None:
-                nbytes = _lib._c_size(0)
-                _lib.check(L.cab_pages_update_workspace_size(self._c, n, nbytes), "cab_pages_update_workspace_size")
-                size = self._sizes[n] = nbytes.value
-            ws = torch.empty(size, dtype=torch.uint8, device=self.device)
-            keep_bytes = keep_stride = keep_cols = num_stride = 0
-            if keep is not None:
-                keep_bytes, keep_stride, keep_cols = keep.element_size(), keep.stride(0), keep.shape[1]
-                num_stride = 0 if keep_num is None else keep_num.stride(0)
-            rc = L.cab_pages_update(self._c, _lib.ptr(src), _lib.ptr(dst), n, _lib.ptr(start), start_value,
-                                    _lib.ptr(keep), keep_bytes, keep_stride, keep_cols, _lib.ptr(keep_num), num_stride,
-                                    _lib.ptr(grow), grow_value, int(copies), ws.data_ptr(), size,
-                                    torch.cuda.current_stream(self.device).cuda_stream)
-            if rc:
-                _lib.check(rc, "cab_pages_update")
+        size = self._sizes.get(n)
+        if size is None:
+            nbytes = _lib._c_size(0)
+            _lib.check(L.cab_pages_update_workspace_size(self._c, n, nbytes), "cab_pages_update_workspace_size")
+            size = self._sizes[n] = nbytes.value
+        ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+        keep_bytes = keep_stride = keep_cols = num_stride = 0
+        if keep is not None:
+            keep_bytes, keep_stride, keep_cols = keep.element_size(), keep.stride(0), keep.shape[1]
+            num_stride = 0 if keep_num is None else keep_num.stride(0)
+        call_on(self.device, "cab_pages_update", L.cab_pages_update, self._c, _lib.ptr(src), _lib.ptr(dst), n,
+                _lib.ptr(start), start_value, _lib.ptr(keep), keep_bytes, keep_stride, keep_cols, _lib.ptr(keep_num),
+                num_stride, _lib.ptr(grow), grow_value, int(copies), ws.data_ptr(), size)
 
     def _rows(self, rows, name: str = "rows"):
         rows = int32_vector(rows, None, name, self.device)
@@ -183,12 +179,8 @@ class PagedKVCache:
             k = k.contiguous()
         if v.stride(3) != 1:
             v = v.contiguous()
-        with on_device(self.device):
-            rc = _lib.lib().cab_pages_write(self._c, layer, k.data_ptr(), v.data_ptr(), n, T, _lib.strides3(k),
-                                            _lib.strides3(v), _lib.ptr(rows), _lib.ptr(num_new), T,
-                                            torch.cuda.current_stream(self.device).cuda_stream)
-            if rc:
-                _lib.check(rc, "cab_pages_write")
+        call_on(self.device, "cab_pages_write", _lib.lib().cab_pages_write, self._c, layer, k.data_ptr(), v.data_ptr(),
+                n, T, _lib.strides3(k), _lib.strides3(v), _lib.ptr(rows), _lib.ptr(num_new), T)
 
     def attend(self, layer: int, q: torch.Tensor, parents: Optional[torch.Tensor] = None,
                tree_mask: Optional[torch.Tensor] = None, num_nodes: Optional[torch.Tensor] = None,

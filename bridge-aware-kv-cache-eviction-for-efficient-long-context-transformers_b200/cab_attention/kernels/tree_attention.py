@@ -55,6 +55,7 @@ def describe_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: to
     c.ref_counts = None if ref_counts is None else ref_counts.data_ptr()
     c.status = None if status is None else status.data_ptr()
     c.dtype = _lib.dtype_code(k_pages)
+    c.sizes = {}  # workspace bytes by call shape
     return c
 
 
@@ -71,19 +72,16 @@ def int32_vector(t: Optional[torch.Tensor], n: Optional[int], name: str, device)
     return t.to(torch.int32).contiguous()
 
 
-class on_device:
-    """Makes ``device`` the current CUDA device for a call, where it is not already."""
-
-    def __init__(self, device: torch.device):
-        self.guard = None if device.index == _current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def call_on(device: torch.device, name: str, fn, *args) -> None:
+    """``fn(*args, stream)`` with ``device`` current, on its current stream."""
+    index = device.index
+    if _current_device() == index:
+        rc = fn(*args, _lib.raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _lib.raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
 
 
 def attend_cache(cache, device, dtype, layer: int, q: torch.Tensor, parents=None, tree_mask=None, num_nodes=None,
@@ -129,22 +127,23 @@ def attend_cache(cache, device, dtype, layer: int, q: torch.Tensor, parents=None
     lse = torch.empty(n, Hq, T, dtype=torch.float32, device=device) if return_lse else None
     if n == 0 or T == 0:
         return (out, lse) if return_lse else out
-    es = q.element_size()
-    if q.stride(3) != 1 or any(s <= 0 or (s * es) % 16 for s in q.stride()[:3]) or q.data_ptr() % 16:
+    qs, es = q.stride(), q.element_size()
+    if qs[3] != 1 or any(x <= 0 or (x * es) % 16 for x in qs[:3]) or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)  # contiguous() would return a misaligned dense view
+        qs = q.stride()
     L = _lib.lib()
-    with on_device(device):
-        nbytes = _lib._c_size(0)
-        rc = L.cab_tree_attn_workspace_size(cache, n, Hq, T, nbytes)
-        if rc:
-            _lib.check(rc, "cab_tree_attn_workspace_size")
-        ws = _lib.workspace(nbytes.value, device)
-        rc = L.cab_tree_attn_fwd(cache, layer, q.data_ptr(), out.data_ptr(), _lib.ptr(lse), n, Hq, T,
-                                 _lib._i64_3(*q.stride()[:3]), _lib._i64_3(*out.stride()[:3]), _lib.ptr(rows),
-                                 _lib.ptr(num_nodes), _lib.ptr(parents), parents_stride, _lib.ptr(tree_mask),
-                                 mask_stride, scale, _lib.ptr(ws), nbytes.value, _lib.stream_of(q))
-        if rc:
-            _lib.check(rc, "cab_tree_attn_fwd")
+    nbytes = cache.sizes.get((n, Hq, T))
+    if nbytes is None:
+        size = _lib._c_size(0)
+        with torch.cuda.device(device.index):
+            _lib.check(L.cab_tree_attn_workspace_size(cache, n, Hq, T, size), "cab_tree_attn_workspace_size")
+        nbytes = cache.sizes[(n, Hq, T)] = size.value
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    os = out.stride()
+    call_on(device, "cab_tree_attn_fwd", L.cab_tree_attn_fwd, cache, layer, q.data_ptr(), out.data_ptr(),
+            None if lse is None else lse.data_ptr(), n, Hq, T, _lib._i64_3(qs[0], qs[1], qs[2]),
+            _lib._i64_3(os[0], os[1], os[2]), _lib.ptr(rows), _lib.ptr(num_nodes), _lib.ptr(parents), parents_stride,
+            _lib.ptr(tree_mask), mask_stride, scale, None if ws is None else ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 
 

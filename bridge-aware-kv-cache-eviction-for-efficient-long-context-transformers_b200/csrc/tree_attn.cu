@@ -307,7 +307,8 @@ constexpr float kRescaleThreshold = 8.0f;
 constexpr int kBufs = 3;
 constexpr uint32_t kTmemO = 384;
 constexpr int kMaxShare = 4;
-constexpr int kWindow = 16;  // tiles whose page numbers the softmax warps check at a time
+constexpr int kLostRing = 16;  // tiles between the K loads and the softmax, at most kStages + 3
+constexpr int kUnitCost = 3;
 constexpr int kWholeTiles = 4;  // rows of at most this many tiles are not cut: no join
 
 template <int D>
@@ -318,7 +319,7 @@ struct Cfg {
   // with as many stages as S / P buffers S(g) completed frees K stage g % 3, PV(g) V stage g % 3
   static constexpr bool kOneSignal = kStages == kBufs;
   static constexpr int kXchg = 2 * 2 * 128 * 4;  // row maxima / sums [parity][key half][row]
-  static constexpr int kBars = (4 * kStages + 3 * kBufs + 3) * 8 + 32;
+  static constexpr int kBars = (4 * kStages + 3 * kBufs + 3) * 8 + 32 + kLostRing;
   static constexpr int kBytes = (1 + 2 * kStages) * kTile + kXchg + kBars;
   static constexpr int kSmem = kBytes + 1024 < 232448 ? kBytes + 1024 : 232448;  // the kernel checks that it fits
   static_assert(kBytes <= 232448, "shared memory");
@@ -339,7 +340,7 @@ __host__ __device__ __forceinline__ Share share_of(int G, int T) {
 }
 
 struct Walk {  // a range of the flat list, unit by unit
-  int b, hk, set, tiles, at;  // tile `at` of the unit's `tiles`
+  int b, hk, set, tiles, at;  // place `at` of the unit's weight; it has `tiles` tiles
   int left;                   // tiles (units, where units stay whole) of the range not yet walked
   Seq s;
 };
@@ -352,19 +353,20 @@ __device__ __forceinline__ int tiles_of(int keys) { return max(1, (keys + 127) /
 __device__ __forceinline__ int unit_tiles(const Params& p, const Share& sh, const Seq& s, int set) {
   return tiles_of(group_keys(p, sh, s, set * sh.wide, min(sh.groups, (set + 1) * sh.wide) - 1));
 }
-// What a unit counts in the flat list, and the units of one KV head of a sequence.
+// What a unit counts in the flat list, and the units of one KV head of a sequence. Starting and
+// ending a unit costs about as much as kUnitCost tiles, which stand before its tiles in the list.
 __device__ __forceinline__ int unit_weight(const Params& p, const Share& sh, const Seq& s, int set) {
-  return p.whole_units ? 1 : unit_tiles(p, sh, s, set);
+  return p.whole_units ? 1 : kUnitCost + unit_tiles(p, sh, s, set);
 }
 __device__ __forceinline__ int head_weight(const Params& p, const Share& sh, const Seq& s) {
   if (p.whole_units) return sh.sets;
   int sum = 0;
-  for (int g = 0; g < sh.sets; ++g) sum += unit_tiles(p, sh, s, g);
+  for (int g = 0; g < sh.sets; ++g) sum += unit_weight(p, sh, s, g);
   return sum;
 }
 
 __device__ __forceinline__ void walk_next(const Params& p, const Share& sh, Walk& w) {  // to the next unit's first tile
-  w.left -= p.whole_units ? 1 : min(w.left, w.tiles - w.at);
+  w.left -= p.whole_units ? 1 : min(w.left, kUnitCost + w.tiles - w.at);
   w.at = 0;
   if (w.left == 0) return;
   if (++w.set == sh.sets) {
@@ -376,11 +378,16 @@ __device__ __forceinline__ void walk_next(const Params& p, const Share& sh, Walk
   }
   w.tiles = unit_tiles(p, sh, w.s, w.set);
 }
-// Tiles of the walk's segment that group grp works on (the unit's longest group has them all).
-__device__ __forceinline__ int own_tiles(const Params& p, const Share& sh, const Walk& w, int grp) {
-  if (grp >= sh.groups) return 0;
-  const int end = min(w.tiles, tiles_of(group_keys(p, sh, w.s, grp, grp)));
-  return max(0, (p.whole_units ? end : min(end, w.at + w.left)) - w.at);
+// The walk's segment: group grp's tiles [first, first + count) (the unit's longest group has them all).
+struct Segment {
+  int first, count;
+};
+__device__ __forceinline__ Segment segment_of(const Params& p, const Share& sh, const Walk& w, int grp) {
+  if (grp >= sh.groups) return Segment{0, 0};
+  const int own = min(w.tiles, tiles_of(group_keys(p, sh, w.s, grp, grp)));
+  if (p.whole_units) return Segment{0, own};
+  const int first = max(0, w.at - kUnitCost), end = min(own, w.at + w.left - kUnitCost);
+  return Segment{first, max(0, end - first)};
 }
 
 __host__ __device__ __forceinline__ int64_t range_start(int64_t total, int64_t ranges, int64_t c) { return total * c / ranges; }
@@ -598,6 +605,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   int* odd_seg = abort_flag + 1;   // the last segment (from 1) whose V tiles held values that are not finite
   int* begin = odd_seg + 1;        // the range: first sequence, weight before it in there, own weight
+  uint8_t* lost = reinterpret_cast<uint8_t*>(begin + 3);  // [kLostRing] tile has a page outside the pool
   {
     uint32_t dyn;
     asm volatile("mov.u32 %0, %%dynamic_smem_size;" : "=r"(dyn));
@@ -617,7 +625,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     prefetch_tensormap(&qmap);
     for (int s = 0; s < 4 * kStages; ++s) mbar_init(&k_full[s], 1);
     for (int s = 0; s < kBufs; ++s) {
-      mbar_init(&s_full[s], 1);
+      mbar_init(&s_full[s], 2);  // the product, and the issuer itself: it passes on what the K loader wrote
       mbar_init(&p_full[s], 8);
       mbar_init(&buf_free[s], 1);
     }
@@ -673,16 +681,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint32_t g = 0, nq = 0;
     bool ok = true;
     for (; w.left > 0 && ok; walk_next(p, sh, w)) {
-      const int T = own_tiles(p, sh, w, w.set * sh.wide + side);
+      const Segment sg = segment_of(p, sh, w, w.set * sh.wide + side);
+      const int T = sg.count;
       if (T == 0) continue;
       const int held = (w.s.len + S - 1) / S;
       const int32_t* row = p.table + w.s.row * p.table_stride;
       // the page of this lane's box in tile i of the segment (the number past the pool: zeros)
       auto page_of = [&](int i) -> int {
-        const int j = (w.at + i) * 128 / S + (S < 128 ? pi : 0);
+        const int j = (sg.first + i) * 128 / S + (S < 128 ? pi : 0);
         if (!mine || i >= T || j >= held) return static_cast<int>(p.pages);
         const int q = row[j];
-        return q < 0 || q >= p.pages ? static_cast<int>(p.pages) : q;
+        return q < 0 || q >= p.pages ? -1 : q;  // -1: a page outside the pool
       };
       int e0 = page_of(0), e1 = page_of(1);  // read two tiles ahead
       if (is_k) {
@@ -708,9 +717,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         ok = mbar_wait(&empty[st], ((g / kStages) & 1) ^ 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&full[st], C::kTile);
+        const bool bad = __any_sync(0xffffffffu, e0 < 0);
+        if (lane == 0) {
+          if (is_k) *reinterpret_cast<volatile uint8_t*>(&lost[g % kLostRing]) = bad;
+          mbar_arrive_expect_tx(&full[st], C::kTile);
+        }
         __syncwarp();
-        if (mine) tma_load_4d(ring + st * C::kTile + off, map, &full[st], 64 * a, S < 128 ? 0 : (w.at + i) * 128 % S, w.hk, e0);
+        if (mine)
+          tma_load_4d(ring + st * C::kTile + off, map, &full[st], 64 * a, S < 128 ? 0 : (sg.first + i) * 128 % S, w.hk,
+                      e0 < 0 ? static_cast<int>(p.pages) : e0);
         __syncwarp();
         e0 = e1;
         e1 = e2;
@@ -730,7 +745,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       uint32_t g = 0, seg = 0;
       bool ok = true;
       for (; w.left > 0 && ok; walk_next(p, sh, w)) {
-        const int T = own_tiles(p, sh, w, w.set * sh.wide + side);
+        const int T = segment_of(p, sh, w, w.set * sh.wide + side).count;
         if (T == 0) continue;
         if (!mbar_wait(q_full, seg & 1, abort_flag)) break;
         ++seg;
@@ -750,6 +765,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           if constexpr (!C::kOneSignal) mma_commit(&k_empty[st]);
           mma_commit(&s_full[buf]);
+          mbar_arrive(&s_full[buf]);
         }
       }
       mma_commit(&drain[0]);
@@ -764,7 +780,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       uint32_t g = 0;
       bool ok = true;
       for (; w.left > 0 && ok; walk_next(p, sh, w)) {
-        const int T = own_tiles(p, sh, w, w.set * sh.wide + side);
+        const int T = segment_of(p, sh, w, w.set * sh.wide + side).count;
         for (int i = 0; i < T; ++i, ++g) {
           const uint32_t st = g % kStages, buf = g % kBufs;
           // V normally lands early; P(g) is the event waited on last. All warps have read the
@@ -797,39 +813,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t t_o = tmem + lanes + kTmemO + kb * (D / 2);
     // tile g's S / P buffer and barrier phase, and its V stage and phase, counted instead of divided
-    uint32_t buf = 0, phase = 0, stage = 0, vphase = 0, xc = 0;
+    uint32_t buf = 0, phase = 0, stage = 0, vphase = 0, xc = 0, tiles_done = 0;
     int seg = 0;
     for (; w.left > 0; walk_next(p, sh, w)) {
       const int grp = w.set * sh.wide + side;
-      const int T = own_tiles(p, sh, w, grp);
+      const Segment sg = segment_of(p, sh, w, grp);
+      const int T = sg.count;
       if (T == 0) continue;
       ++seg;
       const Seq q = w.s;
       const int t = grp * sh.nodes + r / p.G, rows = min(sh.nodes, p.T - grp * sh.nodes) * p.G;
       const bool live = r < rows && t < q.m;
       const bool any_live = __any_sync(0xffffffffu, live);
-      const int key_lo = w.at * 128, keys = group_keys(p, sh, q, grp, grp);
+      const int key_lo = sg.first * 128, keys = group_keys(p, sh, q, grp, grp);
       const bool has_tail = key_lo + T * 128 > q.ctx;
-      const int S = static_cast<int>(p.page_size), held = (q.len + S - 1) / S;
-      // Whether a page of tiles i .. i + kWindow - 1 (this warp's 64 keys of each) is outside the pool.
-      auto lost_pages = [&](int i) -> bool {
-        const int k0 = key_lo + i * 128, j0 = k0 / S, j1 = min(held, (min(k0 + kWindow * 128, key_lo + T * 128) + S - 1) / S);
-        bool lost = false;
-        for (int j = j0 + lane; j < j1; j += 32) {
-          const int pg = p.table[q.row * p.table_stride + j];
-          lost |= pg < 0 || pg >= p.pages;
-        }
-        return __any_sync(0xffffffffu, lost);
-      };
-
       float m_run = -INFINITY, l = 0.f;
       uint32_t before = 0, before_phase = 0;  // the previous tile's buffer
       // One tile, kMasked: some of its keys are nodes, past the length or on a lost page.
       auto tile = [&](auto masked, int i, bool bad) {
         constexpr bool kMasked = decltype(masked)::value;
         const uint32_t t_s = tmem + lanes + buf * 128 + kb * 64;  // S in, P out
-        (void)mbar_wait(&s_full[buf], phase, abort_flag);
-        tc_fence_after_sync();
         uint64_t see = ~0ull;
         if constexpr (kMasked) {
           // S(g) came after PV(g - 3), so V(g)'s barrier is at most this phase behind; P(g) is not
@@ -907,12 +910,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           vphase ^= 1u;
         }
       };
-      const int plain = max(0, min(T, (q.ctx - key_lo) / 128));  // tiles of context alone
-      for (int i0 = 0; i0 < T; i0 += kWindow) {
-        const bool bad = lost_pages(i0);
-        const int i1 = min(T, i0 + kWindow), im = bad ? i0 : min(i1, max(i0, plain));
-        for (int i = i0; i < im; ++i) tile(std::false_type{}, i, false);
-        for (int i = im; i < i1; ++i) tile(std::true_type{}, i, bad);
+      for (int i = 0; i < T; ++i) {
+        (void)mbar_wait(&s_full[buf], phase, abort_flag);
+        tc_fence_after_sync();
+        const bool bad = *reinterpret_cast<volatile uint8_t*>(&lost[tiles_done++ % kLostRing]) != 0;
+        if (!bad && key_lo + (i + 1) * 128 <= q.ctx) tile(std::false_type{}, i, false);
+        else tile(std::true_type{}, i, bad);
       }
 
       // epilogue: the row's two threads take half the columns each
@@ -1015,13 +1018,13 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
     }
     const Seq s = load_seq(p, b);
     before += static_cast<int64_t>(hk) * head_weight(p, sh, s);
-    for (int g = 0; g < set; ++g) before += unit_tiles(p, sh, s, g);
-    const int64_t end = before + tiles_of(group_keys(p, sh, s, grp, grp));
+    for (int g = 0; g < set; ++g) before += unit_weight(p, sh, s, g);
+    const int64_t start = before + kUnitCost, end = start + tiles_of(group_keys(p, sh, s, grp, grp));  // of its tiles
     const int64_t ranges = range_count(total, ctas_max / sh.wide, p.least);
-    // the range of flat tile f is the largest c with total * c / ranges <= f
-    int64_t c0 = (before * ranges + ranges - 1) / total, c1 = ((end - 1) * ranges + ranges - 1) / total;
-    while (range_start(total, ranges, c0) > before) --c0;
-    while (c0 + 1 < ranges && range_start(total, ranges, c0 + 1) <= before) ++c0;
+    // the range of place f is the largest c with total * c / ranges <= f
+    int64_t c0 = (start * ranges + ranges - 1) / total, c1 = ((end - 1) * ranges + ranges - 1) / total;
+    while (range_start(total, ranges, c0) > start) --c0;
+    while (c0 + 1 < ranges && range_start(total, ranges, c0 + 1) <= start) ++c0;
     while (range_start(total, ranges, c1) > end - 1) --c1;
     while (c1 + 1 < ranges && range_start(total, ranges, c1 + 1) <= end - 1) ++c1;
     if (lane == 0) {
