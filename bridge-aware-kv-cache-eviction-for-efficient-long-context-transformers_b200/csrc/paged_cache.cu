@@ -33,9 +33,13 @@ constexpr int kUpdateThreads = 1024;
 constexpr int kMaxPairs = 1024;     // one pair per thread of the prefix sum
 constexpr int64_t kMaxRows = 65536;  // three bitmaps of the rows in shared memory
 constexpr int kMaxCluster = 8;
+constexpr int kFrozen = 1 << 30;     // among the passes: the status word was set before
 
-struct PairRec {
-  int32_t stay, base, start, content;  // R, first rank in the free list, a, C
+// A fresh page: what the copies into it need.
+struct alignas(16) FreshPage {
+  int32_t pair, page;       // pair i and the page's number
+  int32_t first, content;   // its first position in the row, and the row's tokens
+  int32_t start, pad[3];    // a
 };
 
 struct UpdateParams {
@@ -44,17 +48,24 @@ struct UpdateParams {
   const void* keep;
   int64_t start_value, grow_value, keep_stride, keep_cols, keep_num_stride;
   int32_t keep64, n, copies;
-  int32_t* header;     // [0] accepted, [1] fresh pages
-  int32_t* part;       // per CTA of the cluster: first[n] | free | err0 | err1
-  PairRec* pair;       // [n]
-  int32_t* free_list;  // [cap] page of each rank
-  int32_t* rank_pair;  // [cap] pair of each rank
-  int32_t* snap;       // [n, width] the source rows' pages before the update
+  int32_t* header;      // [0] accepted, [1] fresh pages
+  FreshPage* fresh;     // [cap] by rank in the order of taking
+  int32_t* free_list;   // [cap] page of each rank
+  int32_t* snap;        // [n, width] the source rows' pages before the update
   int64_t cap;
 };
 
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// The shared-memory word `p` of CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_word(const void* p, int rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void peer_store(uint32_t a, int32_t v) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+__device__ __forceinline__ void peer_min(uint32_t a, int32_t v) {
+  asm volatile("red.relaxed.cluster.shared::cluster.min.s32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -71,24 +82,6 @@ __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepco
 
 __device__ __forceinline__ int64_t keep_at(const void* keep, int keep64, int64_t off) {
   return keep64 ? static_cast<const int64_t*>(keep)[off] : static_cast<const int32_t*>(keep)[off];
-}
-
-// Sum over the block of one value per thread; every thread gets it. `tmp` holds 33 words.
-__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* tmp) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if (lane == 0) tmp[warp] = v;
-  __syncthreads();
-  if (warp == 0) {
-    int64_t s = lane < static_cast<int>(blockDim.x >> 5) ? tmp[lane] : 0;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) tmp[32] = s;
-  }
-  __syncthreads();
-  return tmp[32];
 }
 
 // Exclusive prefix sum over the block; *total gets the sum.
@@ -119,177 +112,235 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* tmp, int64_t* 
   return tmp[warp] + inc - v;
 }
 
-// One cluster (1 or 8 CTAs) makes the whole update: the work is a few passes over small
-// integer arrays (keep list, use counts, table rows), bound by the latency of its dependent
-// passes, so the passes are separated by cluster barriers instead of launches.
-__global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const UpdateParams p) {
+// One cluster (1 or 8 CTAs) makes the whole update. The work is a few passes over small integer
+// arrays (use counts, keep lists, table rows), bound by the latency of dependent loads, so the
+// passes are separated by cluster barriers instead of launches, what the CTAs tell one another goes through
+// distributed shared memory, and each pass has its loads in flight together.
+constexpr int kWordRounds = 8;  // ballot words of free pages a lane of a warp holds at a time
+
+__global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_constant__ UpdateParams p) {
   extern __shared__ int32_t sh[];
   __shared__ int64_t tmp[33];
-  __shared__ int32_t s_err;
-  grid_launch_dependents();
+  __shared__ int32_t s_err, s_free[kMaxCluster], s_errs[2][kMaxCluster], s_warp_free[32];
   const cab_page_cache& c = p.c;
-  const int n = p.n, tid = threadIdx.x, nt = kUpdateThreads;
+  const int n = p.n, tid = threadIdx.x, nt = kUpdateThreads, lane = tid & 31, warp = tid >> 5;
   const int me = static_cast<int>(cluster_rank()), nc = static_cast<int>(cluster_size());
-  const int64_t S = c.page_size, W = c.width, P = c.pages;
-  int32_t *s_src = sh, *s_dst = sh + n, *s_len = sh + 2 * n, *s_start = sh + 3 * n, *s_content = sh + 4 * n,
-          *s_size = sh + 5 * n, *s_first = sh + 6 * n, *s_stay = sh + 7 * n, *s_base = sh + 8 * n, *s_gone = sh + 9 * n;
+  const int64_t W = c.width, P = c.pages, K = p.keep_cols;
+  const int S = static_cast<int>(c.page_size);
+  int32_t *s_src = sh, *s_dst = sh + n, *s_have = sh + 2 * n, *s_had = sh + 3 * n, *s_start = sh + 4 * n,
+          *s_content = sh + 5 * n, *s_size = sh + 6 * n, *s_first = sh + 7 * n, *s_stay = sh + 8 * n, *s_base = sh + 9 * n,
+          *s_low = sh + 10 * n, *s_room = sh + 11 * n, *s_entry = sh + 12 * n;  // s_entry has n + 1
   const int words = static_cast<int>((c.rows + 31) / 32);
-  uint32_t* b_dst = reinterpret_cast<uint32_t*>(sh + 10 * n);
+  uint32_t* b_dst = reinterpret_cast<uint32_t*>(sh + 13 * n + 1);
   uint32_t *b_src = b_dst + words, *b_multi = b_src + words;
-  const int pstride = n + 3;
-  const bool frozen = *reinterpret_cast<volatile int32_t*>(c.status) != 0;
+  grid_launch_dependents();
 
+  // pass 0: the pairs and their checks (the same in every CTA)
+  int err = *reinterpret_cast<volatile int32_t*>(c.status) != 0 ? kFrozen : 0;
   for (int i = tid; i < 3 * words; i += nt) b_dst[i] = 0u;
   if (tid == 0) s_err = 0;
   __syncthreads();
-  // pass 0: the pairs and their checks (every CTA of the cluster does the same)
   for (int i = tid; i < n; i += nt) {
     const int s = p.src ? p.src[i] : i, d = p.dst ? p.dst[i] : s;
-    int err = 0;
     int64_t len = 0, start = 0, kn = 0, size = 0, gone = 0;
     if (s < 0 || s >= c.rows || d < 0 || d >= c.rows) {
-      err = CAB_PAGES_BAD_ROW;
+      err |= CAB_PAGES_BAD_ROW;
     } else {
       len = c.seq_lens[s];
       gone = c.seq_lens[d];
       start = p.start ? p.start[i] : (p.start_value < 0 ? len : p.start_value);
-      kn = p.keep_num ? p.keep_num[i * p.keep_num_stride] : p.keep_cols;
+      kn = p.keep_num ? p.keep_num[i * p.keep_num_stride] : K;
       const int64_t grow = p.grow ? p.grow[i] : p.grow_value;
-      if (len < 0 || len > W * S || gone < 0 || gone > W * S) err |= CAB_PAGES_BAD_TABLE;
-      else if (start < 0 || start > len || kn < 0 || kn > p.keep_cols || grow < 0) err |= CAB_PAGES_BAD_ARG;
-      else if (start + kn + grow > W * S) err |= CAB_PAGES_TABLE_FULL;
+      int bad = 0;
+      if (len < 0 || len > W * S || gone < 0 || gone > W * S) bad = CAB_PAGES_BAD_TABLE;
+      else if (start < 0 || start > len || kn < 0 || kn > K || grow < 0) bad = CAB_PAGES_BAD_ARG;
+      else if (start + kn + grow > W * S) bad = CAB_PAGES_TABLE_FULL;
       size = start + kn + grow;
-      if (atomicOr(&b_dst[d >> 5], 1u << (d & 31)) >> (d & 31) & 1u) err |= CAB_PAGES_BAD_ROW;
+      if (atomicOr(&b_dst[d >> 5], 1u << (d & 31)) >> (d & 31) & 1u) bad |= CAB_PAGES_BAD_ROW;
       if (atomicOr(&b_src[s >> 5], 1u << (s & 31)) >> (s & 31) & 1u) atomicOr(&b_multi[s >> 5], 1u << (s & 31));
+      if (bad) {
+        err |= bad;
+        len = start = kn = size = gone = 0;
+      }
     }
-    if (err) atomicOr(&s_err, err);
     s_src[i] = s;
     s_dst[i] = d;
-    s_len[i] = static_cast<int32_t>(len);
+    s_have[i] = static_cast<int32_t>((len + S - 1) / S);
+    s_had[i] = static_cast<int32_t>((gone + S - 1) / S);
     s_start[i] = static_cast<int32_t>(start);
     s_content[i] = static_cast<int32_t>(start + kn);
     s_size[i] = static_cast<int32_t>(size);
-    s_gone[i] = static_cast<int32_t>(gone);
     s_first[i] = static_cast<int32_t>(kn);
+    s_room[i] = static_cast<int32_t>(len - start);
   }
-  __syncthreads();
-  const int err0 = s_err;
-  if (frozen || err0) {  // the same in every CTA: nobody waits for the others
-    if (me == 0 && tid == 0) {
-      p.header[0] = 0;
-      if (err0 && !frozen) atomicOr(c.status, err0);
-    }
-    return;
-  }
+  if (err) atomicOr(&s_err, err);
 
-  // pass 1: the keep lists (range, and the first entry that moves) and this CTA's free pages
-  const int64_t K = p.keep_cols;
+  // pass 1: this CTA's free pages: warp w's are lane k's ballot words, `rounds` at a time
+  const int64_t span = ((P + nc - 1) / nc + 31) / 32 * 32, lo = min(P, span * me), hi = min(P, lo + span);
+  const int64_t wspan = (span / 32 + 31) / 32 * 32;  // pages of a warp
+  const int64_t wlo = min(hi, lo + wspan * warp), whi = min(hi, wlo + wspan);
+  uint32_t held_words = 0u;  // lane k: ballot of the warp's pages 32 k .. 32 k + 31 (the first 1024)
+  int warp_free = 0;
+  for (int64_t q0 = wlo; q0 < whi; q0 += 32 * kWordRounds) {
+    int32_t refs[kWordRounds];
+#pragma unroll
+    for (int u = 0; u < kWordRounds; ++u) {
+      const int64_t q = q0 + 32 * u + lane;
+      refs[u] = q < whi ? c.ref_counts[q] : 1;
+    }
+#pragma unroll
+    for (int u = 0; u < kWordRounds; ++u) {
+      const uint32_t word = __ballot_sync(0xffffffffu, refs[u] == 0);
+      if ((q0 - wlo) / 32 + u == lane) held_words = word;
+      warp_free += __popc(word);
+    }
+  }
+  if (lane == 0) s_warp_free[warp] = warp_free;
+  __syncthreads();  // the pairs and the warps' counts are there
+  cluster_arrive();  // the peers may write into this CTA's shared memory from here on
+  // the keep lists: range, and the first entry that moves
   if (K > 0) {
-    int bad = 0;
+    bool bad = false;
     const int64_t total = K * n;
     for (int64_t e = static_cast<int64_t>(me) * nt + tid; e < total; e += static_cast<int64_t>(nc) * nt) {
       const int i = static_cast<int>(e / K);
-      const int64_t x = e - i * K;
+      const int x = static_cast<int>(e - i * K);
       if (x < s_content[i] - s_start[i]) {
         const int64_t v = keep_at(p.keep, p.keep64, i * p.keep_stride + x);
-        if (v < 0 || v >= s_len[i] - s_start[i]) bad = 1;
-        if (v != x && x < *reinterpret_cast<volatile int32_t*>(&s_first[i])) atomicMin(&s_first[i], static_cast<int32_t>(x));
+        bad |= v < 0 || v >= s_room[i];
+        if (v != x && x < *reinterpret_cast<volatile int32_t*>(&s_first[i])) atomicMin(&s_first[i], x);
       }
     }
     if (bad) atomicOr(&s_err, CAB_PAGES_BAD_ARG);
+    __syncthreads();
   }
-  const int64_t span = (P + nc - 1) / nc;
-  const int64_t lo = min(P, span * me), hi = min(P, span * (me + 1));
-  int64_t mine = 0;
-  for (int64_t q = lo + tid; q < hi; q += nt) mine += c.ref_counts[q] == 0;
-  const int64_t free_here = block_sum(mine, tmp);  // its barriers also complete s_first and s_err
-  int32_t* part = p.part + static_cast<int64_t>(me) * pstride;
-  for (int i = tid; i < n; i += nt) part[i] = s_first[i];
-  if (tid == 0) {
-    part[n] = static_cast<int32_t>(free_here);
-    part[n + 1] = s_err;
-    s_err = 0;
+  cluster_wait();
+  if (tid < nc) {
+    int f = 0;
+    for (int k = 0; k < 32; ++k) f += s_warp_free[k];
+    peer_store(peer_word(&s_free[me], tid), f);
+    peer_store(peer_word(&s_errs[0][me], tid), s_err);
   }
-  cluster_sync_all();
+  if (K > 0 && nc > 1)
+    for (int i = tid; i < n; i += nt) {
+      const int f = s_first[i];
+      if (f < s_content[i] - s_start[i])
+        for (int k = 0; k < nc; ++k) peer_min(peer_word(&s_first[i], k), f);
+    }
+  cluster_arrive();
+  cluster_wait();
 
-  // pass 2: what stays, what is fresh (every CTA the same); the free list and the snapshot
+  // pass 2: what stays, what is fresh (the same in every CTA); the source rows before the update
   int64_t free_total = 0, free_before = 0;
-  int err1 = 0;
+  err = 0;
   for (int k = 0; k < nc; ++k) {
-    const int32_t* q = p.part + static_cast<int64_t>(k) * pstride;
-    const int32_t f = __ldcg(q + n);
-    if (k < me) free_before += f;
-    free_total += f;
-    err1 |= __ldcg(q + n + 1);
+    if (k < me) free_before += s_free[k];
+    free_total += s_free[k];
+    err |= s_errs[0][k];
   }
-  int64_t need = 0;
+  if (err) {  // the same in every CTA
+    if (me == 0 && tid == 0) {
+      p.header[0] = 0;
+      if (!(err & kFrozen)) atomicOr(c.status, err);
+    }
+    return;
+  }
+  if (tid == 0) s_err = 0;
+  int64_t need = 0, entries = 0;
+  bool shared_tail = false;
   if (tid < n) {
-    const int i = tid;
-    int32_t first = s_content[i] - s_start[i];
-    for (int k = 0; k < nc; ++k) first = min(first, __ldcg(p.part + static_cast<int64_t>(k) * pstride + i));
-    const int64_t intact = static_cast<int64_t>(s_start[i]) + first, held = s_content[i];
-    int64_t stay = intact / S;
-    const int s = s_src[i];
-    if (intact == held && held % S != 0 && s == s_dst[i]) {
+    const int i = tid, s = s_src[i];
+    const bool in_place = s == s_dst[i];
+    const int held = s_content[i], intact = s_start[i] + s_first[i];
+    int stay = intact / S;
+    if (intact == held && held % S != 0 && in_place) {
       const int32_t tail = c.block_table[s * c.table_stride + held / S];
       const bool alone = tail >= 0 && tail < P && c.ref_counts[tail] == 1 && !(b_multi[s >> 5] >> (s & 31) & 1u);
       if (alone) ++stay;
-      else if (!p.copies) atomicOr(&s_err, CAB_PAGES_BAD_TABLE);  // a shared last page and no copy asked for
+      else shared_tail = !p.copies;  // a last page in use elsewhere and no copy asked for
     }
-    s_stay[i] = static_cast<int32_t>(stay);
-    need = (static_cast<int64_t>(s_size[i]) + S - 1) / S - stay;
+    const int now = static_cast<int>((static_cast<int64_t>(s_size[i]) + S - 1) / S);
+    s_stay[i] = stay;
+    need = now - stay;
+    // entries [low, high) of the rows are looked at: all of the source's where copies or shares need them
+    const bool all = !in_place || K > 0;
+    const int low = all ? 0 : stay, high = max(max(s_had[i], now), all ? s_have[i] : 0);
+    s_low[i] = low;
+    entries = max(0, high - low);
   }
-  int64_t total = 0;
-  const int64_t base = block_scan(need, tmp, &total);
+  int64_t sums = 0;
+  const int64_t at = block_scan(need << 32 | entries, tmp, &sums);  // both sums are below 2^31
+  const int64_t total = sums >> 32, all_entries = sums & 0x7fffffff;
   if (tid < n) {
-    s_base[tid] = static_cast<int32_t>(base);
-    if (me == 0) p.pair[tid] = PairRec{s_stay[tid], static_cast<int32_t>(base), s_start[tid], s_content[tid]};
+    s_base[tid] = static_cast<int32_t>(at >> 32);
+    s_entry[tid] = static_cast<int32_t>(at & 0x7fffffff);
   }
-  if (total > free_total) err1 |= CAB_PAGES_FULL;
-  if (free_before < total && total <= free_total) {
-    int64_t rank0 = free_before;
-    for (int64_t q0 = lo; q0 < hi && rank0 < total; q0 += nt) {
-      const int64_t q = q0 + tid;
-      int64_t got = 0;
-      const int64_t is_free = q < hi && c.ref_counts[q] == 0;
-      const int64_t r = rank0 + block_scan(is_free, tmp, &got);
-      if (is_free && r < total) p.free_list[r] = static_cast<int32_t>(q);
-      rank0 += got;
-    }
-  }
+  if (tid == 0) s_entry[n] = static_cast<int32_t>(all_entries);
+  if (shared_tail) atomicOr(&s_err, CAB_PAGES_BAD_TABLE);
   __syncthreads();
-  // Rows are walked in 32-entry chunks by warps of the whole cluster; the same thread later
-  // rewrites the entry it has read here.
-  const int64_t cpr = (W + 31) / 32, chunks = cpr * n;
-  const int lane = tid & 31;
-  const int64_t w0 = (static_cast<int64_t>(me) * nt + tid) >> 5, wn = static_cast<int64_t>(nc) * nt / 32;
-  for (int64_t ch = w0; ch < chunks; ch += wn) {
-    const int i = static_cast<int>(ch / cpr);
-    const int64_t j = (ch - i * cpr) * 32 + lane;
-    const bool in_place = s_src[i] == s_dst[i];
-    const int64_t have = (static_cast<int64_t>(s_len[i]) + S - 1) / S;
-    int bad = 0;
-    if (j < have && (!in_place || K > 0 || j >= s_stay[i])) {
-      const int32_t q = c.block_table[s_src[i] * c.table_stride + j];
-      p.snap[static_cast<int64_t>(i) * W + j] = q;
-      bad |= q < 0 || q >= P;
+  if (total > free_total) {
+    err = CAB_PAGES_FULL;
+  } else if (free_before < total) {
+    int64_t rank = free_before;
+    for (int k = 0; k < warp; ++k) rank += s_warp_free[k];
+    for (int64_t q0 = wlo; q0 < whi && rank < total; q0 += 32) {
+      const int k = static_cast<int>((q0 - wlo) / 32);
+      const uint32_t word = k < 32 ? __shfl_sync(0xffffffffu, held_words, k)
+                                   : __ballot_sync(0xffffffffu, q0 + lane < whi && c.ref_counts[q0 + lane] == 0);
+      const int64_t r = rank + __popc(word & ((1u << lane) - 1u));
+      if (word >> lane & 1u && r < total) p.free_list[r] = static_cast<int32_t>(q0 + lane);
+      rank += __popc(word);
     }
-    if (!in_place && j < (static_cast<int64_t>(s_gone[i]) + S - 1) / S) {
-      const int32_t q = c.block_table[s_dst[i] * c.table_stride + j];
-      bad |= q < 0 || q >= P;
-    }
-    if (bad) atomicOr(&s_err, CAB_PAGES_BAD_TABLE);
   }
+  constexpr int kRound = 4;
+  const int64_t first_entry = static_cast<int64_t>(me) * nt + tid, step = static_cast<int64_t>(nc) * nt;
+  auto pair_of = [&](int e) {  // the pair whose entries hold e
+    int a = 0, b = n;
+    while (b - a > 1) {
+      const int m = (a + b) >> 1;
+      if (s_entry[m] <= e) a = m;
+      else b = m;
+    }
+    return a;
+  };
+  bool bad = false;
+  for (int64_t e0 = first_entry; e0 < all_entries; e0 += step * kRound) {
+    int32_t from[kRound], gone[kRound];
+    int64_t to[kRound];
+#pragma unroll
+    for (int u = 0; u < kRound; ++u) {
+      const int64_t e = e0 + step * u;
+      from[u] = gone[u] = 0;
+      to[u] = -1;
+      if (e < all_entries) {
+        const int i = pair_of(static_cast<int>(e)), j = s_low[i] + static_cast<int>(e) - s_entry[i];
+        const int s = s_src[i], d = s_dst[i];
+        if (j < s_have[i]) {
+          from[u] = c.block_table[s * c.table_stride + j];
+          to[u] = static_cast<int64_t>(i) * W + j;
+        }
+        if (s != d && j < s_had[i]) gone[u] = c.block_table[d * c.table_stride + j];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kRound; ++u) {
+      if (to[u] >= 0) p.snap[to[u]] = from[u];
+      bad |= from[u] < 0 || from[u] >= P || gone[u] < 0 || gone[u] >= P;
+    }
+  }
+  if (bad) atomicOr(&s_err, CAB_PAGES_BAD_TABLE);
   __syncthreads();
-  if (tid == 0) part[n + 2] = s_err;
-  cluster_sync_all();
+  if (tid < nc) peer_store(peer_word(&s_errs[1][me], tid), s_err | err);
+  cluster_arrive();
+  cluster_wait();
 
   // pass 3: refuse, or apply
-  for (int k = 0; k < nc; ++k) err1 |= __ldcg(p.part + static_cast<int64_t>(k) * pstride + n + 2);
-  if (err1) {
+  err = 0;
+  for (int k = 0; k < nc; ++k) err |= s_errs[1][k];
+  if (err) {
     if (me == 0 && tid == 0) {
       p.header[0] = 0;
-      atomicOr(c.status, err1);
+      atomicOr(c.status, err);
     }
     return;
   }
@@ -297,24 +348,42 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const UpdateP
     p.header[0] = 1;
     p.header[1] = static_cast<int32_t>(total);
   }
-  for (int64_t ch = w0; ch < chunks; ch += wn) {
-    const int i = static_cast<int>(ch / cpr);
-    const int64_t j = (ch - i * cpr) * 32 + lane;
-    const bool in_place = s_src[i] == s_dst[i];
-    const int64_t had = (static_cast<int64_t>(s_gone[i]) + S - 1) / S, now = (static_cast<int64_t>(s_size[i]) + S - 1) / S;
-    if (j >= max(had, now) || (in_place && j < s_stay[i])) continue;
-    int32_t* entry = c.block_table + s_dst[i] * c.table_stride + j;
-    if (j < had) atomicSub(&c.ref_counts[*entry], 1);
-    int32_t q = -1;
-    if (j < s_stay[i]) {
-      q = p.snap[static_cast<int64_t>(i) * W + j];
-    } else if (j < now) {
-      const int32_t r = s_base[i] + static_cast<int32_t>(j - s_stay[i]);
-      q = __ldcg(p.free_list + r);
-      p.rank_pair[r] = i;
+  for (int64_t e0 = first_entry; e0 < all_entries; e0 += step * kRound) {
+    int32_t old[kRound], now_page[kRound];
+    int32_t* entry[kRound];
+#pragma unroll
+    for (int u = 0; u < kRound; ++u) {
+      const int64_t e = e0 + step * u;
+      old[u] = now_page[u] = -1;
+      entry[u] = nullptr;
+      if (e < all_entries) {
+        const int i = pair_of(static_cast<int>(e)), j = s_low[i] + static_cast<int>(e) - s_entry[i];
+        const int now = static_cast<int>((static_cast<int64_t>(s_size[i]) + S - 1) / S);
+        const bool in_place = s_src[i] == s_dst[i];
+        if (j < max(s_had[i], now) && !(in_place && j < s_stay[i])) {
+          entry[u] = c.block_table + s_dst[i] * c.table_stride + j;
+          if (j < s_had[i]) old[u] = *entry[u];
+          if (j < s_stay[i]) {
+            now_page[u] = p.snap[static_cast<int64_t>(i) * W + j];
+          } else if (j < now) {
+            const int r = s_base[i] + j - s_stay[i];
+            now_page[u] = __ldcg(p.free_list + r);
+            if (p.copies) {
+              int4* f = reinterpret_cast<int4*>(p.fresh + r);
+              f[0] = make_int4(i, now_page[u], j * S, s_content[i]);
+              f[1] = make_int4(s_start[i], 0, 0, 0);
+            }
+          }
+        }
+      }
     }
-    if (q >= 0) atomicAdd(&c.ref_counts[q], 1);
-    *entry = q;
+#pragma unroll
+    for (int u = 0; u < kRound; ++u)
+      if (entry[u] != nullptr) {
+        if (old[u] >= 0) atomicSub(&c.ref_counts[old[u]], 1);
+        if (now_page[u] >= 0) atomicAdd(&c.ref_counts[now_page[u]], 1);
+        *entry[u] = now_page[u];
+      }
   }
   if (me == 0)
     for (int i = tid; i < n; i += nt) c.seq_lens[s_dst[i]] = s_size[i];
@@ -365,32 +434,30 @@ __device__ __forceinline__ void move_rows(const V* __restrict__ ksrc, const V* _
 }
 
 template <typename V>
-__global__ void __launch_bounds__(256) copy_kernel(const UpdateParams p, int vec_elems, int vecs) {
-  grid_dependency_wait();
-  if (p.header[0] == 0) return;
+__global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ UpdateParams p, int vec_elems, int vecs) {
   const cab_page_cache& c = p.c;
-  const int total = p.header[1];
-  const int64_t S = c.page_size, W = c.width;
-  const int groups = static_cast<int>((S + 31) / 32);
-  const int64_t lh = c.layers * c.heads, tasks = static_cast<int64_t>(total) * groups * lh;
+  const int S = static_cast<int>(c.page_size), groups = (S + 31) / 32;
+  const int lh = static_cast<int>(c.layers * c.heads), heads = static_cast<int>(c.heads);
   const int lane = threadIdx.x & 31;
   const int64_t wn = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
-  for (int64_t task = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); task < tasks; task += wn) {
+  int64_t task = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  grid_dependency_wait();
+  if (p.header[0] == 0) return;
+  const int64_t tasks = static_cast<int64_t>(p.header[1]) * groups * lh;
+  for (; task < tasks; task += wn) {
     const int64_t rg = task / lh;
-    const int x = static_cast<int>(task - rg * lh);
-    const int l = x / static_cast<int>(c.heads), h = x - l * static_cast<int>(c.heads);
+    const int x = static_cast<int>(task - rg * lh), l = x / heads, h = x - l * heads;
     const int r = static_cast<int>(rg / groups), g = static_cast<int>(rg - static_cast<int64_t>(r) * groups);
-    const int i = p.rank_pair[r];
-    const PairRec pr = p.pair[i];
-    const int64_t pos0 = (static_cast<int64_t>(pr.stay) + r - pr.base) * S + 32 * g;
-    const int count = static_cast<int>(min(min(static_cast<int64_t>(32), S - 32 * g), pr.content - pos0));
+    const int4 f = *reinterpret_cast<const int4*>(p.fresh + r);
+    const int start = p.fresh[r].start;
+    const int pos0 = f.z + 32 * g, count = min(min(32, S - 32 * g), f.w - pos0);
     if (count <= 0) continue;
     RowSpan m{0, 0, -1, -1};
     if (lane < count) {
-      const int64_t pos = pos0 + lane;
-      const int64_t from = pos < pr.start ? pos : pr.start + keep_at(p.keep, p.keep64, i * p.keep_stride + pos - pr.start);
-      const int64_t pg = p.snap[static_cast<int64_t>(i) * W + from / S], slot = from % S;
-      const int64_t to = p.free_list[r], ts = 32 * g + lane;
+      const int pos = pos0 + lane;
+      const int from = pos < start ? pos : start + static_cast<int>(keep_at(p.keep, p.keep64, f.x * p.keep_stride + pos - start));
+      const int64_t pg = p.snap[static_cast<int64_t>(f.x) * c.width + from / S], slot = from % S;
+      const int64_t to = f.y, ts = 32 * g + lane;
       const int64_t kb = l * c.k_strides[0] + h * c.k_strides[2], vb = l * c.v_strides[0] + h * c.v_strides[2];
       m.ksrc = (kb + pg * c.k_strides[1] + slot * c.k_strides[3]) / vec_elems;
       m.vsrc = (vb + pg * c.v_strides[1] + slot * c.v_strides[3]) / vec_elems;
@@ -412,7 +479,7 @@ struct WriteParams {
 };
 
 template <typename V>
-__global__ void __launch_bounds__(256) write_kernel(const WriteParams p, int vec_elems, int vecs) {
+__global__ void __launch_bounds__(256) write_kernel(const __grid_constant__ WriteParams p, int vec_elems, int vecs) {
   const cab_page_cache& c = p.c;
   if (*reinterpret_cast<volatile int32_t*>(c.status) != 0) return;
   const int64_t S = c.page_size;
@@ -492,7 +559,7 @@ inline int vector_bytes(const cab_page_cache* c, const void* k, const void* v, c
 }
 
 struct UpdateLayout {
-  size_t part, pair, free_list, rank_pair, snap, total;
+  size_t fresh, free_list, snap, total;
   int64_t cap;
 };
 
@@ -500,13 +567,17 @@ inline UpdateLayout update_layout(const cab_page_cache* c, int64_t n) {
   auto up = [](size_t x) { return (x + 15) & ~size_t(15); };
   UpdateLayout L{};
   L.cap = std::min(c->pages, n * c->width);
-  L.part = 16;
-  L.pair = up(L.part + static_cast<size_t>(kMaxCluster) * (n + 3) * 4);
-  L.free_list = up(L.pair + static_cast<size_t>(n) * sizeof(PairRec));
-  L.rank_pair = up(L.free_list + static_cast<size_t>(L.cap) * 4);
-  L.snap = up(L.rank_pair + static_cast<size_t>(L.cap) * 4);
+  L.fresh = 16;
+  L.free_list = L.fresh + static_cast<size_t>(L.cap) * sizeof(FreshPage);
+  L.snap = up(L.free_list + static_cast<size_t>(L.cap) * 4);
   L.total = up(L.snap + static_cast<size_t>(n) * c->width * 4);
   return L;
+}
+
+inline int check_pairs(const cab_page_cache* c, int64_t n) {
+  if (n <= 0 || n > kMaxPairs) return fail(CAB_ERR_UNSUPPORTED, "pages_update: 1 to %d pairs a call, got %lld", kMaxPairs, (long long)n);
+  if (n * c->width >= (int64_t)1 << 31) return fail(CAB_ERR_UNSUPPORTED, "pages_update: more than 2^31 table entries a call");
+  return CAB_OK;
 }
 
 }  // namespace pages
@@ -517,7 +588,7 @@ extern "C" int cab_pages_update_workspace_size(const cab_page_cache* cache, int6
   using namespace cab::pages;
   if (!bytes) return fail(CAB_ERR_INVALID_ARG, "pages_update_workspace_size: NULL output");
   if (int rc = check_cache(cache, "pages_update_workspace_size", false)) return rc;
-  if (n <= 0 || n > kMaxPairs) return fail(CAB_ERR_UNSUPPORTED, "pages_update: 1 to %d pairs a call, got %lld", kMaxPairs, (long long)n);
+  if (int rc = check_pairs(cache, n)) return rc;
   *bytes = update_layout(cache, n).total;
   return CAB_OK;
 }
@@ -530,7 +601,7 @@ extern "C" int cab_pages_update(const cab_page_cache* cache, const int32_t* src,
   using namespace cab;
   using namespace cab::pages;
   if (int rc = check_cache(cache, "pages_update", copies != 0)) return rc;
-  if (n <= 0 || n > kMaxPairs) return fail(CAB_ERR_UNSUPPORTED, "pages_update: 1 to %d pairs a call, got %lld", kMaxPairs, (long long)n);
+  if (int rc = check_pairs(cache, n)) return rc;
   if (!src && n > cache->rows) return fail(CAB_ERR_INVALID_ARG, "pages_update: %lld pairs without source rows, %lld rows", (long long)n, (long long)cache->rows);
   if (keep_cols < 0 || keep_cols >= (int64_t)1 << 31) return fail(CAB_ERR_INVALID_ARG, "pages_update: bad number of keep columns");
   if (keep_cols > 0 && (!keep || (keep_bytes != 4 && keep_bytes != 8))) return fail(CAB_ERR_INVALID_ARG, "pages_update: keep must be int32 or int64");
@@ -558,21 +629,20 @@ extern "C" int cab_pages_update(const cab_page_cache* cache, const int32_t* src,
   p.n = static_cast<int32_t>(n);
   p.copies = copies != 0;
   p.header = reinterpret_cast<int32_t*>(ws);
-  p.part = reinterpret_cast<int32_t*>(ws + L.part);
-  p.pair = reinterpret_cast<PairRec*>(ws + L.pair);
+  p.fresh = reinterpret_cast<FreshPage*>(ws + L.fresh);
   p.free_list = reinterpret_cast<int32_t*>(ws + L.free_list);
-  p.rank_pair = reinterpret_cast<int32_t*>(ws + L.rank_pair);
   p.snap = reinterpret_cast<int32_t*>(ws + L.snap);
   p.cap = L.cap;
 
   const int64_t words = (cache->rows + 31) / 32;
-  const size_t smem = static_cast<size_t>(10 * n + 3 * words) * 4;
+  const size_t smem = static_cast<size_t>(13 * n + 1 + 3 * words) * 4;
   if (smem > 40 * 1024)
     cudaFuncSetAttribute(update_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  const int64_t ints = cache->pages + n * (cache->width + keep_cols);
+  // one CTA reads up to 8 values a thread of each array in one go; more are spread over a cluster
+  const int64_t ints = std::max(cache->pages, n * std::max(cache->width, keep_cols));
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(ints > 16384 ? kMaxCluster : 1);
+  cfg.gridDim = dim3(ints > 8 * kUpdateThreads ? kMaxCluster : 1);
   cfg.blockDim = dim3(kUpdateThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
@@ -588,8 +658,8 @@ extern "C" int cab_pages_update(const cab_page_cache* cache, const int32_t* src,
   const int vb = vector_bytes(cache, nullptr, nullptr, nullptr, nullptr);
   const int es = static_cast<int>(dtype_size(static_cast<int>(cache->dtype)));
   const int vecs = static_cast<int>(cache->dim * es / vb), ve = vb >= es ? vb / es : 1;
-  // at most keep_cols + page_size tokens of a pair move, or one page where nothing is listed
-  const int64_t per = keep_cols > 0 ? (keep_cols + cache->page_size - 1) / cache->page_size + 1 : cache->width;
+  // without a list only a pair's last page is copied, else at most keep_cols + page_size tokens
+  const int64_t per = keep_cols > 0 ? (keep_cols + cache->page_size - 1) / cache->page_size + 1 : 1;
   const int64_t most = std::min(L.cap, n * std::min(per, cache->width)) * ((cache->page_size + 31) / 32) * cache->layers * cache->heads;
   cudaLaunchConfig_t cc{};
   cudaLaunchAttribute ca[1];
