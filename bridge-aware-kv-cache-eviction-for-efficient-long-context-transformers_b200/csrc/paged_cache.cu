@@ -48,6 +48,7 @@ struct UpdateParams {
   const void* keep;
   int64_t start_value, grow_value, keep_stride, keep_cols, keep_num_stride;
   int32_t keep64, n, copies;
+  uint32_t div_mul, div_shift;  // x / page_size = x * div_mul >> div_shift for x < 2^31
   int32_t* header;      // [0] accepted, [1] fresh pages
   FreshPage* fresh;     // [cap] by rank in the order of taking
   int32_t* free_list;   // [cap] page of each rank
@@ -55,8 +56,14 @@ struct UpdateParams {
   int64_t cap;
 };
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// A barrier over the cluster's CTAs (one CTA needs only its own).
+__device__ __forceinline__ void cluster_sync(int nc) {
+  if (nc == 1) {
+    __syncthreads();
+    return;
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // The shared-memory word `p` of CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t peer_word(const void* p, int rank) {
   uint32_t a;
@@ -64,8 +71,10 @@ __device__ __forceinline__ uint32_t peer_word(const void* p, int rank) {
   return a;
 }
 __device__ __forceinline__ void peer_store(uint32_t a, int32_t v) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
-__device__ __forceinline__ void peer_min(uint32_t a, int32_t v) {
-  asm volatile("red.relaxed.cluster.shared::cluster.min.s32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+__device__ __forceinline__ int32_t peer_load(uint32_t a) {
+  int32_t v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -80,12 +89,17 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// x / page_size by a multiplication: a hardware-free 32-bit division costs some 150 clocks each time.
+__device__ __forceinline__ uint32_t pages_before(const UpdateParams& p, uint32_t x) {
+  return static_cast<uint32_t>(static_cast<uint64_t>(x) * p.div_mul >> p.div_shift);
+}
+
 __device__ __forceinline__ int64_t keep_at(const void* keep, int keep64, int64_t off) {
   return keep64 ? static_cast<const int64_t*>(keep)[off] : static_cast<const int32_t*>(keep)[off];
 }
 
-// Exclusive prefix sum over the block; *total gets the sum.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* tmp, int64_t* total) {
+// Exclusive prefix sum over the first n threads' values (0 beyond); *total gets the sum.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int n, int64_t* tmp, int64_t* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t inc = v;
 #pragma unroll
@@ -93,7 +107,12 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* tmp, int64_t* 
     const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += u;
   }
-  __syncthreads();
+  if (n <= 32) {  // all in warp 0
+    if (threadIdx.x == 31) tmp[32] = inc;
+    __syncthreads();
+    *total = tmp[32];
+    return inc - v;
+  }
   if (lane == 31) tmp[warp] = inc;
   __syncthreads();
   if (warp == 0) {
@@ -116,22 +135,22 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* tmp, int64_t* 
 // arrays (use counts, keep lists, table rows), bound by the latency of dependent loads, so the
 // passes are separated by cluster barriers instead of launches, what the CTAs tell one another goes through
 // distributed shared memory, and each pass has its loads in flight together.
-constexpr int kWordRounds = 8;  // ballot words of free pages a lane of a warp holds at a time
+constexpr int kWordRounds = 2;  // ballot words of free pages a lane of a warp holds at a time
 
 __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_constant__ UpdateParams p) {
   extern __shared__ int32_t sh[];
   __shared__ int64_t tmp[33];
-  __shared__ int32_t s_err, s_free[kMaxCluster], s_errs[2][kMaxCluster], s_warp_free[32];
+  __shared__ int32_t s_err, s_told[2], s_free[kMaxCluster], s_errs[kMaxCluster], s_late[kMaxCluster], s_warp_free[32];
   const cab_page_cache& c = p.c;
   const int n = p.n, tid = threadIdx.x, nt = kUpdateThreads, lane = tid & 31, warp = tid >> 5;
   const int me = static_cast<int>(cluster_rank()), nc = static_cast<int>(cluster_size());
   const int64_t W = c.width, P = c.pages, K = p.keep_cols;
-  const int S = static_cast<int>(c.page_size);
+  const uint32_t S = static_cast<uint32_t>(c.page_size);  // lengths and W * S are below 2^31
   int32_t *s_src = sh, *s_dst = sh + n, *s_have = sh + 2 * n, *s_had = sh + 3 * n, *s_start = sh + 4 * n,
           *s_content = sh + 5 * n, *s_size = sh + 6 * n, *s_first = sh + 7 * n, *s_stay = sh + 8 * n, *s_base = sh + 9 * n,
-          *s_low = sh + 10 * n, *s_room = sh + 11 * n, *s_entry = sh + 12 * n;  // s_entry has n + 1
+          *s_low = sh + 10 * n, *s_room = sh + 11 * n, *s_alone = sh + 12 * n, *s_now = sh + 13 * n, *s_entry = sh + 14 * n;  // s_entry has n + 1
   const int words = static_cast<int>((c.rows + 31) / 32);
-  uint32_t* b_dst = reinterpret_cast<uint32_t*>(sh + 13 * n + 1);
+  uint32_t* b_dst = reinterpret_cast<uint32_t*>(sh + 15 * n + 1);
   uint32_t *b_src = b_dst + words, *b_multi = b_src + words;
   grid_launch_dependents();
 
@@ -142,15 +161,17 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
   __syncthreads();
   for (int i = tid; i < n; i += nt) {
     const int s = p.src ? p.src[i] : i, d = p.dst ? p.dst[i] : s;
+    const int64_t start_i = p.start ? p.start[i] : p.start_value, keep_i = p.keep_num ? p.keep_num[i * p.keep_num_stride] : K,
+                  grow = p.grow ? p.grow[i] : p.grow_value;
     int64_t len = 0, start = 0, kn = 0, size = 0, gone = 0;
+    bool alone = false;
     if (s < 0 || s >= c.rows || d < 0 || d >= c.rows) {
       err |= CAB_PAGES_BAD_ROW;
     } else {
       len = c.seq_lens[s];
       gone = c.seq_lens[d];
-      start = p.start ? p.start[i] : (p.start_value < 0 ? len : p.start_value);
-      kn = p.keep_num ? p.keep_num[i * p.keep_num_stride] : K;
-      const int64_t grow = p.grow ? p.grow[i] : p.grow_value;
+      start = !p.start && start_i < 0 ? len : start_i;
+      kn = keep_i;
       int bad = 0;
       if (len < 0 || len > W * S || gone < 0 || gone > W * S) bad = CAB_PAGES_BAD_TABLE;
       else if (start < 0 || start > len || kn < 0 || kn > K || grow < 0) bad = CAB_PAGES_BAD_ARG;
@@ -161,12 +182,17 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
       if (bad) {
         err |= bad;
         len = start = kn = size = gone = 0;
+      } else if (const uint32_t held = static_cast<uint32_t>(start + kn), full = pages_before(p, held); s == d && full * S != held) {
+        // in place with a partly filled last page: whether it is this row's alone
+        const int32_t tail = c.block_table[s * c.table_stride + full];
+        alone = tail >= 0 && tail < P && c.ref_counts[tail] == 1;
       }
     }
+    s_alone[i] = alone;
     s_src[i] = s;
     s_dst[i] = d;
-    s_have[i] = static_cast<int32_t>((len + S - 1) / S);
-    s_had[i] = static_cast<int32_t>((gone + S - 1) / S);
+    s_have[i] = static_cast<int32_t>(pages_before(p, static_cast<uint32_t>(len) + S - 1));
+    s_had[i] = static_cast<int32_t>(pages_before(p, static_cast<uint32_t>(gone) + S - 1));
     s_start[i] = static_cast<int32_t>(start);
     s_content[i] = static_cast<int32_t>(start + kn);
     s_size[i] = static_cast<int32_t>(size);
@@ -197,7 +223,6 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
   }
   if (lane == 0) s_warp_free[warp] = warp_free;
   __syncthreads();  // the pairs and the warps' counts are there
-  cluster_arrive();  // the peers may write into this CTA's shared memory from here on
   // the keep lists: range, and the first entry that moves
   if (K > 0) {
     bool bad = false;
@@ -214,21 +239,24 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
     if (bad) atomicOr(&s_err, CAB_PAGES_BAD_ARG);
     __syncthreads();
   }
-  cluster_wait();
-  if (tid < nc) {
-    int f = 0;
-    for (int k = 0; k < 32; ++k) f += s_warp_free[k];
-    peer_store(peer_word(&s_free[me], tid), f);
-    peer_store(peer_word(&s_errs[0][me], tid), s_err);
-  }
-  if (K > 0 && nc > 1)
-    for (int i = tid; i < n; i += nt) {
-      const int f = s_first[i];
-      if (f < s_content[i] - s_start[i])
-        for (int k = 0; k < nc; ++k) peer_min(peer_word(&s_first[i], k), f);
+  if (warp == 0) {
+    int f = s_warp_free[lane];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) f += __shfl_xor_sync(0xffffffffu, f, o);
+    if (lane == 0) {
+      s_told[0] = f;
+      s_told[1] = s_err;
     }
-  cluster_arrive();
-  cluster_wait();
+  }
+  cluster_sync(nc);
+  if (tid < nc) {
+    s_free[tid] = peer_load(peer_word(&s_told[0], tid));
+    s_errs[tid] = peer_load(peer_word(&s_told[1], tid));
+  }
+  int first = tid < n ? s_first[tid] : 0;
+  if (K > 0 && tid < n)
+    for (int k = 1; k < nc; ++k) first = min(first, peer_load(peer_word(&s_first[tid], (me + k) % nc)));
+  __syncthreads();
 
   // pass 2: what stays, what is fresh (the same in every CTA); the source rows before the update
   int64_t free_total = 0, free_before = 0;
@@ -236,9 +264,10 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
   for (int k = 0; k < nc; ++k) {
     if (k < me) free_before += s_free[k];
     free_total += s_free[k];
-    err |= s_errs[0][k];
+    err |= s_errs[k];
   }
-  if (err) {  // the same in every CTA
+  if (err) {  // the same in every CTA; a peer may still read this one's words
+    cluster_sync(nc);
     if (me == 0 && tid == 0) {
       p.header[0] = 0;
       if (!(err & kFrozen)) atomicOr(c.status, err);
@@ -251,15 +280,14 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
   if (tid < n) {
     const int i = tid, s = s_src[i];
     const bool in_place = s == s_dst[i];
-    const int held = s_content[i], intact = s_start[i] + s_first[i];
-    int stay = intact / S;
-    if (intact == held && held % S != 0 && in_place) {
-      const int32_t tail = c.block_table[s * c.table_stride + held / S];
-      const bool alone = tail >= 0 && tail < P && c.ref_counts[tail] == 1 && !(b_multi[s >> 5] >> (s & 31) & 1u);
-      if (alone) ++stay;
+    const uint32_t held = s_content[i], intact = s_start[i] + first;
+    int stay = static_cast<int>(pages_before(p, intact));
+    if (intact == held && stay * S != held && in_place) {
+      if (s_alone[i] && !(b_multi[s >> 5] >> (s & 31) & 1u)) ++stay;
       else shared_tail = !p.copies;  // a last page in use elsewhere and no copy asked for
     }
-    const int now = static_cast<int>((static_cast<int64_t>(s_size[i]) + S - 1) / S);
+    const int now = static_cast<int>(pages_before(p, static_cast<uint32_t>(s_size[i]) + S - 1));
+    s_now[i] = now;
     s_stay[i] = stay;
     need = now - stay;
     // entries [low, high) of the rows are looked at: all of the source's where copies or shares need them
@@ -269,7 +297,7 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
     entries = max(0, high - low);
   }
   int64_t sums = 0;
-  const int64_t at = block_scan(need << 32 | entries, tmp, &sums);  // both sums are below 2^31
+  const int64_t at = block_scan(need << 32 | entries, n, tmp, &sums);  // both sums are below 2^31
   const int64_t total = sums >> 32, all_entries = sums & 0x7fffffff;
   if (tid < n) {
     s_base[tid] = static_cast<int32_t>(at >> 32);
@@ -292,51 +320,48 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
       rank += __popc(word);
     }
   }
-  constexpr int kRound = 4;
+  // The entries of all rows, spread over the cluster's threads, kRound of a thread's loads in flight. What a
+  // thread has read of its last round (its only one, up to kRound * 8192 entries) it keeps for pass 3.
+  constexpr int kRound = 2;
   const int64_t first_entry = static_cast<int64_t>(me) * nt + tid, step = static_cast<int64_t>(nc) * nt;
-  auto pair_of = [&](int e) {  // the pair whose entries hold e
+  const bool one_round = all_entries <= step * kRound;
+  int pair[kRound], col[kRound], from[kRound], gone[kRound];
+  auto place = [&](int64_t e, int& i, int& j) {  // the pair whose entries hold e, and the column
     int a = 0, b = n;
     while (b - a > 1) {
       const int m = (a + b) >> 1;
       if (s_entry[m] <= e) a = m;
       else b = m;
     }
-    return a;
+    i = e < all_entries ? a : -1;
+    j = s_low[a] + static_cast<int>(e) - s_entry[a];
   };
   bool bad = false;
   for (int64_t e0 = first_entry; e0 < all_entries; e0 += step * kRound) {
-    int32_t from[kRound], gone[kRound];
-    int64_t to[kRound];
 #pragma unroll
     for (int u = 0; u < kRound; ++u) {
-      const int64_t e = e0 + step * u;
+      place(e0 + step * u, pair[u], col[u]);
+      const int i = pair[u], j = col[u];
       from[u] = gone[u] = 0;
-      to[u] = -1;
-      if (e < all_entries) {
-        const int i = pair_of(static_cast<int>(e)), j = s_low[i] + static_cast<int>(e) - s_entry[i];
-        const int s = s_src[i], d = s_dst[i];
-        if (j < s_have[i]) {
-          from[u] = c.block_table[s * c.table_stride + j];
-          to[u] = static_cast<int64_t>(i) * W + j;
-        }
-        if (s != d && j < s_had[i]) gone[u] = c.block_table[d * c.table_stride + j];
+      if (i >= 0) {
+        if (j < s_have[i]) from[u] = c.block_table[s_src[i] * c.table_stride + j];
+        if (j < s_had[i]) gone[u] = c.block_table[s_dst[i] * c.table_stride + j];
       }
     }
 #pragma unroll
     for (int u = 0; u < kRound; ++u) {
-      if (to[u] >= 0) p.snap[to[u]] = from[u];
+      if (pair[u] >= 0 && p.copies && col[u] < s_have[pair[u]]) p.snap[static_cast<int64_t>(pair[u]) * W + col[u]] = from[u];
       bad |= from[u] < 0 || from[u] >= P || gone[u] < 0 || gone[u] >= P;
     }
   }
   if (bad) atomicOr(&s_err, CAB_PAGES_BAD_TABLE);
   __syncthreads();
-  if (tid < nc) peer_store(peer_word(&s_errs[1][me], tid), s_err | err);
-  cluster_arrive();
-  cluster_wait();
+  if (tid < nc) peer_store(peer_word(&s_late[me], tid), s_err | err);
+  cluster_sync(nc);
 
   // pass 3: refuse, or apply
   err = 0;
-  for (int k = 0; k < nc; ++k) err |= s_errs[1][k];
+  for (int k = 0; k < nc; ++k) err |= s_late[k];
   if (err) {
     if (me == 0 && tid == 0) {
       p.header[0] = 0;
@@ -349,40 +374,37 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
     p.header[1] = static_cast<int32_t>(total);
   }
   for (int64_t e0 = first_entry; e0 < all_entries; e0 += step * kRound) {
-    int32_t old[kRound], now_page[kRound];
-    int32_t* entry[kRound];
+    int32_t page[kRound];
+    bool write[kRound];
 #pragma unroll
     for (int u = 0; u < kRound; ++u) {
-      const int64_t e = e0 + step * u;
-      old[u] = now_page[u] = -1;
-      entry[u] = nullptr;
-      if (e < all_entries) {
-        const int i = pair_of(static_cast<int>(e)), j = s_low[i] + static_cast<int>(e) - s_entry[i];
-        const int now = static_cast<int>((static_cast<int64_t>(s_size[i]) + S - 1) / S);
-        const bool in_place = s_src[i] == s_dst[i];
-        if (j < max(s_had[i], now) && !(in_place && j < s_stay[i])) {
-          entry[u] = c.block_table + s_dst[i] * c.table_stride + j;
-          if (j < s_had[i]) old[u] = *entry[u];
-          if (j < s_stay[i]) {
-            now_page[u] = p.snap[static_cast<int64_t>(i) * W + j];
-          } else if (j < now) {
-            const int r = s_base[i] + j - s_stay[i];
-            now_page[u] = __ldcg(p.free_list + r);
-            if (p.copies) {
-              int4* f = reinterpret_cast<int4*>(p.fresh + r);
-              f[0] = make_int4(i, now_page[u], j * S, s_content[i]);
-              f[1] = make_int4(s_start[i], 0, 0, 0);
-            }
-          }
+      if (!one_round) place(e0 + step * u, pair[u], col[u]);
+      const int i = pair[u], j = col[u];
+      page[u] = -1;
+      write[u] = false;
+      if (i >= 0) {
+        const int now = s_now[i];
+        write[u] = j < max(s_had[i], now) && !(s_src[i] == s_dst[i] && j < s_stay[i]);
+        if (!one_round && write[u]) {
+          if (j < s_had[i]) gone[u] = c.block_table[s_dst[i] * c.table_stride + j];
+          if (j < s_stay[i]) from[u] = p.snap[static_cast<int64_t>(i) * W + j];
         }
+        if (write[u] && j < s_stay[i]) page[u] = from[u];
+        else if (write[u] && j < now) page[u] = __ldcg(p.free_list + s_base[i] + j - s_stay[i]);
       }
     }
 #pragma unroll
     for (int u = 0; u < kRound; ++u)
-      if (entry[u] != nullptr) {
-        if (old[u] >= 0) atomicSub(&c.ref_counts[old[u]], 1);
-        if (now_page[u] >= 0) atomicAdd(&c.ref_counts[now_page[u]], 1);
-        *entry[u] = now_page[u];
+      if (write[u]) {
+        const int i = pair[u], j = col[u];
+        if (j < s_had[i]) atomicSub(&c.ref_counts[gone[u]], 1);
+        if (page[u] >= 0) atomicAdd(&c.ref_counts[page[u]], 1);
+        c.block_table[s_dst[i] * c.table_stride + j] = page[u];
+        if (p.copies && page[u] >= 0 && j >= s_stay[i]) {
+          int4* f = reinterpret_cast<int4*>(p.fresh + s_base[i] + j - s_stay[i]);
+          f[0] = make_int4(i, page[u], static_cast<int>(j * S), s_content[i]);
+          f[1] = make_int4(s_start[i], 0, 0, 0);
+        }
       }
   }
   if (me == 0)
@@ -441,15 +463,15 @@ __global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ Updat
   const int lane = threadIdx.x & 31;
   const int64_t wn = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
   int64_t task = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int64_t most = p.cap * groups * lh;
   grid_dependency_wait();
-  if (p.header[0] == 0) return;
-  const int64_t tasks = static_cast<int64_t>(p.header[1]) * groups * lh;
-  for (; task < tasks; task += wn) {
+  for (; task < most; task += wn) {
     const int64_t rg = task / lh;
     const int x = static_cast<int>(task - rg * lh), l = x / heads, h = x - l * heads;
     const int r = static_cast<int>(rg / groups), g = static_cast<int>(rg - static_cast<int64_t>(r) * groups);
-    const int4 f = *reinterpret_cast<const int4*>(p.fresh + r);
+    const int4 f = *reinterpret_cast<const int4*>(p.fresh + r);  // read along with the header: r is within it
     const int start = p.fresh[r].start;
+    if (p.header[0] == 0 || r >= p.header[1]) return;
     const int pos0 = f.z + 32 * g, count = min(min(32, S - 32 * g), f.w - pos0);
     if (count <= 0) continue;
     RowSpan m{0, 0, -1, -1};
@@ -531,7 +553,7 @@ inline int check_cache(const cab_page_cache* c, const char* what, bool data, boo
     return fail(CAB_ERR_INVALID_ARG, "%s: NULL pointer in the cache", what);
   if (c->layers <= 0 || c->pages <= 0 || c->heads <= 0 || c->page_size <= 0 || c->dim <= 0 || c->rows <= 0 || c->width <= 0)
     return fail(CAB_ERR_INVALID_ARG, "%s: non-positive size in the cache", what);
-  if (c->pages >= (int64_t)1 << 31 || c->rows > kMaxRows || c->width * c->page_size >= (int64_t)1 << 31 ||
+  if (c->pages >= (int64_t)1 << 31 || c->rows > kMaxRows || (c->width + 1) * c->page_size >= (int64_t)1 << 31 ||
       c->layers * c->heads >= (int64_t)1 << 31)
     return fail(CAB_ERR_UNSUPPORTED, "%s: cache too large (at most 2^31 - 1 pages, 65536 rows, 2^31 - 1 tokens a row)", what);
   if (c->table_stride < c->width && c->rows > 1) return fail(CAB_ERR_INVALID_ARG, "%s: table rows overlap", what);
@@ -633,9 +655,13 @@ extern "C" int cab_pages_update(const cab_page_cache* cache, const int32_t* src,
   p.free_list = reinterpret_cast<int32_t*>(ws + L.free_list);
   p.snap = reinterpret_cast<int32_t*>(ws + L.snap);
   p.cap = L.cap;
+  uint32_t log2s = 0;
+  while ((int64_t)1 << log2s < cache->page_size) ++log2s;
+  p.div_mul = static_cast<uint32_t>((((uint64_t)1 << (31 + log2s)) + cache->page_size - 1) / cache->page_size);
+  p.div_shift = 31 + log2s;
 
   const int64_t words = (cache->rows + 31) / 32;
-  const size_t smem = static_cast<size_t>(13 * n + 1 + 3 * words) * 4;
+  const size_t smem = static_cast<size_t>(15 * n + 1 + 3 * words) * 4;
   if (smem > 40 * 1024)
     cudaFuncSetAttribute(update_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   // one CTA reads up to 8 values a thread of each array in one go; more are spread over a cluster
