@@ -59,6 +59,7 @@ struct Params {
   int32_t part_rows;  // rows of a partial slot
   int32_t out_vec;    // out rows start on 16 bytes
   int32_t whole_units;  // no unit is cut: none can be longer than a few tiles
+  int32_t in_vec;       // CUDA-core path: K / V rows can be read 4 elements at a time
   float *part_o, *part_ml;
 };
 
@@ -105,116 +106,216 @@ __device__ __forceinline__ int key_limit(const Params& p, const Seq& s, int t_la
 
 // ------------------------------------------------------------------ CUDA-core path
 // fp32 arithmetic for any type, page size and head_dim <= 256: float32 caches, and shapes the
-// tensor-core path does not take. One CTA per (sequence, KV head, 16 rows, key split); a warp
-// owns 4 rows, a lane one key of the 32-key tile for the scores and a set of columns for the
-// output, so the row maximum and sum stay in the warp.
-constexpr int kRowsTile = 16, kKeysTile = 32, kSimtThreads = 128;
+// tensor-core path does not take. One CTA per (sequence, KV head, 4 * RW rows, key split). A warp
+// owns RW rows and a lane one key of the 32-key tile for the scores, so a row's maximum and sum are
+// warp reductions; for the output a lane owns the columns lane + 32 c. Four threads fetch a key: its page is
+// looked up once, then its K and V rows come in 4-element vectors. Bound by shared-memory reads: per 4 dims
+// 4 wavefronts of keys and one of each row's query for 4 * RW multiply-adds, so many rows take RW = 8, few
+// (up to 16) RW = 4 to spread them over the warps.
+constexpr int kKeysTile = 32, kSimtThreads = 128;
 
-template <typename T, int DC>
-__global__ void __launch_bounds__(kSimtThreads) simt_kernel(const Params p) {
+template <typename T>
+struct Vec4;
+template <>
+struct Vec4<float> {
+  using type = float4;
+  static __device__ __forceinline__ float4 widen(float4 v) { return v; }
+};
+template <>
+struct Vec4<__half> {
+  using type = uint2;
+  static __device__ __forceinline__ float4 widen(uint2 v) {
+    const float2 a = __half22float2(*reinterpret_cast<__half2*>(&v.x)), b = __half22float2(*reinterpret_cast<__half2*>(&v.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+};
+template <>
+struct Vec4<__nv_bfloat16> {
+  using type = uint2;
+  static __device__ __forceinline__ float4 widen(uint2 v) {
+    const float2 a = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v.x)),
+                 b = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+};
+
+template <typename T, int DC, int RW>
+__global__ void __launch_bounds__(kSimtThreads) simt_kernel(const __grid_constant__ Params p) {
   extern __shared__ float sm[];
+  constexpr int kRowsTile = 4 * RW;
+  using V4 = typename Vec4<T>::type;
   const int Dp = (p.D + 3) & ~3, ld = Dp + 4;
-  float* sQ = sm;                    // [16][Dp]
+  float* sQ = sm;                    // [rows][Dp]
   float* sK = sQ + kRowsTile * Dp;   // [32][ld]
   float* sV = sK + kKeysTile * ld;   // [32][Dp]
+  float* sP = sV + kKeysTile * Dp;   // [rows][32]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int R = p.G * p.T, tiles_r = (R + kRowsTile - 1) / kRowsTile;
   const int unit = blockIdx.x, split = blockIdx.y;
   const int rt = unit % tiles_r, hk = (unit / tiles_r) % p.Hkv, i = unit / (tiles_r * p.Hkv);
   const int row0 = rt * kRowsTile;
   const Seq s = load_seq(p, i);
-  const int keys = s.m > 0 ? key_limit(p, s, min(p.T - 1, (row0 + kRowsTile - 1) / p.G)) : 0;
+  const int keys = s.m > 0 && row0 / p.G < s.m ? key_limit(p, s, min(p.T - 1, (row0 + kRowsTile - 1) / p.G)) : 0;
   const int tiles = (keys + kKeysTile - 1) / kKeysTile;
   const int per = (tiles + p.splits - 1) / p.splits;
   const int t_lo = min(tiles, split * per), t_hi = min(tiles, t_lo + per);
+  const uint32_t S = static_cast<uint32_t>(p.page_size);
+  const int32_t* table = p.table + s.row * p.table_stride;
+  // the key this thread fetches a quarter of
+  const int fk = threadIdx.x >> 2, part = threadIdx.x & 3;
+  auto page_at = [&](int tile) -> int {  // of that key; -1: none
+    const int key = tile * kKeysTile + fk;
+    if (tile >= t_hi || key >= keys) return -1;
+    const int pg = table[static_cast<uint32_t>(key) / S];
+    return pg < 0 || pg >= p.pages ? -1 : pg;
+  };
+  int page = page_at(t_lo);
 
-  for (int e = threadIdx.x; e < kRowsTile * Dp; e += kSimtThreads) {
-    const int r = e / Dp, d = e - r * Dp, row = row0 + r;
-    float x = 0.f;
-    if (row < R && d < p.D)
-      x = to_f32(static_cast<const T*>(p.q)[i * p.qs[0] + (hk * p.G + row % p.G) * p.qs[1] + (row / p.G) * p.qs[2] + d]);
-    sQ[e] = x;
-  }
-  float acc[4][DC], m[4], l[4];
+  {
+    float q[RW][DC];  // this warp's rows, all in flight
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < RW; ++r) {
+      const int row = row0 + warp * RW + r, t = row / p.G;
+      const T* src = static_cast<const T*>(p.q) + i * p.qs[0] + (hk * p.G + row - t * p.G) * p.qs[1] + t * p.qs[2];
+#pragma unroll
+      for (int c = 0; c < DC; ++c) q[r][c] = row < R && lane + 32 * c < p.D ? to_f32(src[lane + 32 * c]) : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < RW; ++r)
+#pragma unroll
+      for (int c = 0; c < DC; ++c)
+        if (lane + 32 * c < Dp) sQ[(warp * RW + r) * Dp + lane + 32 * c] = q[r][c];
+  }
+  float acc[RW][DC], m[RW], l[RW];
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.f;
 #pragma unroll
     for (int c = 0; c < DC; ++c) acc[r][c] = 0.f;
   }
-  const int32_t* table = p.table + s.row * p.table_stride;
   for (int tile = t_lo; tile < t_hi; ++tile) {
     const int key0 = tile * kKeysTile;
+    const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);  // four lanes a key
+    const int next_page = page_at(tile + 1);
     __syncthreads();
-    for (int e = threadIdx.x; e < kKeysTile * Dp; e += kSimtThreads) {
-      const int j = e / Dp, d = e - j * Dp, key = key0 + j;
-      float a = 0.f, b = 0.f;
-      if (key < keys && d < p.D) {
-        const int64_t pg = table[key / p.page_size], slot = key % p.page_size;
-        if (pg >= 0 && pg < p.pages) {
-          a = to_f32(static_cast<const T*>(p.k)[pg * p.ks[0] + hk * p.ks[1] + slot * p.ks[2] + d]);
-          b = to_f32(static_cast<const T*>(p.v)[pg * p.vs[0] + hk * p.vs[1] + slot * p.vs[2] + d]);
+    if (lane < 8) reinterpret_cast<uint32_t*>(sP)[warp * 8 + lane] = there >> (4 * lane) & 1u;  // before P is written
+    {
+      const int64_t slot = static_cast<uint32_t>(key0 + fk) % S;
+      const T* k = static_cast<const T*>(p.k) + page * p.ks[0] + hk * p.ks[1] + slot * p.ks[2];
+      const T* v = static_cast<const T*>(p.v) + page * p.vs[0] + hk * p.vs[1] + slot * p.vs[2];
+      float* dk = sK + fk * ld;
+      float* dv = sV + fk * Dp;
+      if (p.in_vec) {
+        constexpr int kChunks = DC * 2;  // 32 DC columns, 4 threads of 4
+        V4 a[kChunks], b[kChunks];
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const int d = 16 * c + 4 * part;
+          if (page >= 0 && d < p.D) {
+            a[c] = *reinterpret_cast<const V4*>(k + d);
+            b[c] = *reinterpret_cast<const V4*>(v + d);
+          } else {
+            a[c] = b[c] = V4{};
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const int d = 16 * c + 4 * part;
+          if (d < Dp) {
+            *reinterpret_cast<float4*>(dk + d) = Vec4<T>::widen(a[c]);
+            *reinterpret_cast<float4*>(dv + d) = Vec4<T>::widen(b[c]);
+          }
+        }
+      } else {
+        for (int d = part; d < Dp; d += 4) {
+          const bool ok = page >= 0 && d < p.D;
+          dk[d] = ok ? to_f32(k[d]) : 0.f;
+          dv[d] = ok ? to_f32(v[d]) : 0.f;
         }
       }
-      sK[j * ld + d] = a;
-      sV[j * Dp + d] = b;
     }
+    page = next_page;
     __syncthreads();
-    float sc[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool key_there = reinterpret_cast<const uint32_t*>(sP)[lane] != 0u;
+    float sc[RW];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) sc[r] = 0.f;
     const float4* kr = reinterpret_cast<const float4*>(sK + lane * ld);
+    const float4* qr = reinterpret_cast<const float4*>(sQ + warp * RW * Dp);
+#pragma unroll 4
     for (int d = 0; d < Dp / 4; ++d) {
       const float4 kk = kr[d];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float4 qq = reinterpret_cast<const float4*>(sQ + (warp * 4 + r) * Dp)[d];
+      for (int r = 0; r < RW; ++r) {
+        const float4 qq = qr[r * (Dp / 4) + d];
         sc[r] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, sc[r]))));
       }
     }
     const int key = key0 + lane;
-    bool there = key < keys;
-    if (there) {
-      const int64_t pg = table[key / p.page_size];
-      there = pg >= 0 && pg < p.pages;
-    }
-    uint32_t seen[4];
-    float pr[4];
+    uint32_t seen[RW], all = 0xffffffffu;
+    __syncthreads();  // every warp has read the keys' flags
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int t = (row0 + warp * 4 + r) / p.G;
-      const bool ok = there && t < s.m && (key < s.ctx || sees(p, i, t, key - s.ctx));
+    for (int r = 0; r < RW; ++r) {
+      const int t = (row0 + warp * RW + r) / p.G;
+      const bool ok = key_there && t < s.m && (key < s.ctx || (key < keys && sees(p, i, t, key - s.ctx)));
       seen[r] = __ballot_sync(0xffffffffu, ok);
-      float x = ok ? sc[r] * p.scale_log2 : -INFINITY, mx = x;
+      all &= seen[r];
+      const float x = ok ? sc[r] * p.scale_log2 : -INFINITY;
+      float mx = x;
 #pragma unroll
       for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       const float mn = fmaxf(m[r], mx);
       const float alpha = m[r] == -INFINITY ? 0.f : ex2(m[r] - mn);
-      pr[r] = x == -INFINITY ? 0.f : ex2(x - mn);  // unseen, or a score of -inf
-      float sum = pr[r];
-#pragma unroll
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      l[r] = l[r] * alpha + sum;
+      const float w = x == -INFINITY ? 0.f : ex2(x - mn);  // unseen, or a score of -inf
+      l[r] = l[r] * alpha + w;                             // this lane's keys; the lanes are added at the end
       m[r] = mn;
+      sP[(warp * RW + r) * 32 + lane] = w;
+      if (alpha != 1.f) {
 #pragma unroll
-      for (int c = 0; c < DC; ++c) acc[r][c] *= alpha;
+        for (int c = 0; c < DC; ++c) acc[r][c] *= alpha;
+      }
     }
-    for (int j = 0; j < kKeysTile; ++j) {
-      float vv[DC];
+    __syncwarp();
+    const float4* pr = reinterpret_cast<const float4*>(sP + warp * RW * 32);
+    if (all == 0xffffffffu) {
+#pragma unroll 2
+      for (int j = 0; j < kKeysTile; j += 4) {
+        float vv[4][DC];
 #pragma unroll
-      for (int c = 0; c < DC; ++c) vv[c] = lane + 32 * c < Dp ? sV[j * Dp + lane + 32 * c] : 0.f;
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float w = __shfl_sync(0xffffffffu, pr[r], j);
-        if (seen[r] >> j & 1u) {
+          for (int c = 0; c < DC; ++c) vv[u][c] = lane + 32 * c < Dp ? sV[(j + u) * Dp + lane + 32 * c] : 0.f;
 #pragma unroll
-          for (int c = 0; c < DC; ++c) acc[r][c] = fmaf(w, vv[c], acc[r][c]);
+        for (int r = 0; r < RW; ++r) {
+          const float4 w = pr[r * 8 + j / 4];
+#pragma unroll
+          for (int c = 0; c < DC; ++c)
+            acc[r][c] = fmaf(w.x, vv[0][c], fmaf(w.y, vv[1][c], fmaf(w.z, vv[2][c], fmaf(w.w, vv[3][c], acc[r][c]))));
+        }
+      }
+    } else {  // unseen keys are left out, not multiplied by 0
+      for (int j = 0; j < kKeysTile; ++j) {
+        float vv[DC];
+#pragma unroll
+        for (int c = 0; c < DC; ++c) vv[c] = lane + 32 * c < Dp ? sV[j * Dp + lane + 32 * c] : 0.f;
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+          if (seen[r] >> j & 1u) {
+            const float w = sP[(warp * RW + r) * 32 + j];
+#pragma unroll
+            for (int c = 0; c < DC; ++c) acc[r][c] = fmaf(w, vv[c], acc[r][c]);
+          }
         }
       }
     }
   }
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int row = row0 + warp * 4 + r;
+  for (int r = 0; r < RW; ++r) {
+    const int row = row0 + warp * RW + r;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
     if (row >= R) continue;
     if (p.splits == 1) {
       const int h = hk * p.G + row % p.G, t = row / p.G;
@@ -225,49 +326,56 @@ __global__ void __launch_bounds__(kSimtThreads) simt_kernel(const Params p) {
         if (lane + 32 * c < p.D) o[lane + 32 * c] = from_f32<T>(acc[r][c] * inv);
       if (p.lse && lane == 0) p.lse[(static_cast<int64_t>(i) * p.Hq + h) * p.T + t] = (m[r] + log2f(l[r])) * kLn2;
     } else {
-      const int64_t slot = (static_cast<int64_t>(unit) * p.splits + split) * kRowsTile + warp * 4 + r;
+      const int64_t slot = (static_cast<int64_t>(unit) * kRowsTile + warp * RW + r) * p.splits + split;
 #pragma unroll
       for (int c = 0; c < DC; ++c)
         if (lane + 32 * c < p.D) p.part_o[slot * p.D + lane + 32 * c] = acc[r][c];
-      if (lane == 0) {
-        p.part_ml[slot * 2] = m[r];
-        p.part_ml[slot * 2 + 1] = l[r];
-      }
+      if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m[r], l[r]);
     }
   }
 }
 
-// Joins the splits of a row: one warp per row, always in the order of the keys.
+// Joins the splits of a row: one warp per row, always in the order of the keys. The splits'
+// weights are computed by a lane each, so the sums' loads do not wait for one another.
 template <typename T, int DC>
-__global__ void __launch_bounds__(kSimtThreads) simt_join_kernel(const Params p) {
+__global__ void __launch_bounds__(kSimtThreads) simt_join_kernel(const __grid_constant__ Params p, int rows_tile) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int R = p.G * p.T, tiles_r = (R + kRowsTile - 1) / kRowsTile;
-  const int64_t total = static_cast<int64_t>(p.n) * p.Hkv * tiles_r * kRowsTile;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int R = p.G * p.T, tiles_r = (R + rows_tile - 1) / rows_tile;
+  const int64_t total = static_cast<int64_t>(p.n) * p.Hkv * tiles_r * rows_tile;
   const int64_t x = static_cast<int64_t>(blockIdx.x) * 4 + warp;
-  if (x >= total) return;
-  const int64_t unit = x / kRowsTile;
-  const int r = static_cast<int>(x - unit * kRowsTile);
+  const int64_t unit = x / rows_tile;
   const int rt = static_cast<int>(unit % tiles_r), hk = static_cast<int>(unit / tiles_r % p.Hkv);
   const int64_t i = unit / tiles_r / p.Hkv;
-  const int row = rt * kRowsTile + r;
-  if (row >= R) return;
-  float m = -INFINITY;
-  for (int k = lane; k < p.splits; k += 32) m = fmaxf(m, p.part_ml[((unit * p.splits + k) * kRowsTile + r) * 2]);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float acc[DC], l = 0.f;
+  const int row = rt * rows_tile + static_cast<int>(x - unit * rows_tile);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (x >= total || row >= R) return;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + x * p.splits;
+  const float* po = p.part_o + x * p.splits * p.D;
+  float m = -INFINITY, l = 0.f, acc[DC];
 #pragma unroll
   for (int c = 0; c < DC; ++c) acc[c] = 0.f;
-  for (int k = 0; k < p.splits; ++k) {
-    const int64_t slot = (unit * p.splits + k) * kRowsTile + r;
-    const float mk = p.part_ml[slot * 2], lk = p.part_ml[slot * 2 + 1];
-    if (mk == -INFINITY && lk == 0.f) continue;
-    const float w = ex2(mk - m);
-    l = fmaf(w, lk, l);
+  for (int k0 = 0; k0 < p.splits; k0 += 32) {
+    const float2 own = k0 + lane < p.splits ? ml[k0 + lane] : make_float2(-INFINITY, 0.f);
+    float mx = own.x;
 #pragma unroll
-    for (int c = 0; c < DC; ++c)
-      if (lane + 32 * c < p.D) acc[c] = fmaf(w, p.part_o[slot * p.D + lane + 32 * c], acc[c]);
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
+    const float alpha = ex2(m - ref), w = own.x == -INFINITY && own.y == 0.f ? 0.f : ex2(own.x - ref);
+    float lw = w * own.y;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, o);
+    l = fmaf(l, alpha, lw);
+    m = mn;
+#pragma unroll
+    for (int c = 0; c < DC; ++c) acc[c] *= alpha;
+    const int n = min(32, p.splits - k0);
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+#pragma unroll
+      for (int c = 0; c < DC; ++c)
+        if (lane + 32 * c < p.D) acc[c] = fmaf(wk, po[static_cast<int64_t>(k0 + k) * p.D + lane + 32 * c], acc[c]);
+    }
   }
   const int h = hk * p.G + row % p.G, t = row / p.G;
   T* o = static_cast<T*>(p.out) + i * p.os[0] + h * p.os[1] + t * p.os[2];
@@ -486,28 +594,32 @@ __device__ __forceinline__ void fix_up(const Params& p, const Seq& s, int b, int
 // that are not finite do. Returns whether there were any.
 template <int D, bool kBF16>
 __device__ __forceinline__ bool clean_v_row(uint8_t* tile, int r, int half, int key, const Seq& s) {
-  constexpr uint32_t kExp = kBF16 ? 0x7F80u : 0x7C00u;
-  bool found = false;
+  constexpr uint32_t kExp = kBF16 ? 0x7F807F80u : 0x7C007C00u, kOne = kBF16 ? 0x00800080u : 0x04000400u;
+  const int x0 = half * (D / 16);  // first 16-byte chunk of the row
+  auto chunk = [&](int x) { return reinterpret_cast<uint4*>(tile + (x >> 3) * 16384 + sw128_offset(r, x & 7)); };
+  if (key >= s.len) {
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) *chunk(x0 + c) = make_uint4(0, 0, 0, 0);
+    return false;
+  }
+  uint32_t hit = 0u;  // an exponent of ones carries into the bit above it
 #pragma unroll
   for (int c = 0; c < D / 16; ++c) {
-    const int x = half * (D / 16) + c;  // 16-byte chunk of the row
-    uint4* q = reinterpret_cast<uint4*>(tile + (x >> 3) * 16384 + sw128_offset(r, x & 7));
-    if (key >= s.len) {
-      *q = make_uint4(0, 0, 0, 0);
-      continue;
-    }
-    uint4 v = *q;
-    uint32_t* e = reinterpret_cast<uint32_t*>(&v);
-    bool hit = false;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if ((e[k] & kExp) == kExp) { e[k] &= 0xFFFF0000u; hit = true; }
-      if ((e[k] & (kExp << 16)) == (kExp << 16)) { e[k] &= 0x0000FFFFu; hit = true; }
-    }
-    if (hit) *q = v;
-    found |= hit;
+    const uint4 v = *chunk(x0 + c);
+    hit |= ((v.x & kExp) + kOne) | ((v.y & kExp) + kOne) | ((v.z & kExp) + kOne) | ((v.w & kExp) + kOne);
   }
-  return found;
+  if ((hit & 0x80008000u) == 0u) return false;
+  for (int c = 0; c < D / 16; ++c) {
+    uint4 v = *chunk(x0 + c);
+    uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t h = ((e[k] & kExp) + kOne) & 0x80008000u;
+      if (h & 0x8000u) e[k] &= 0xFFFF0000u;
+      if (h & 0x80000000u) e[k] &= 0x0000FFFFu;
+    }
+    *chunk(x0 + c) = v;
+  }
+  return true;
 }
 
 template <bool kBF16>
@@ -552,25 +664,20 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return r;
 }
 
-// Up to 64 weights of a row's half tile from its scores s[64] (in place), kMasked: only those of
-// the bits `see`. Writes P and returns their sum.
-template <bool kBF16, bool kMasked>
-__device__ __forceinline__ float weights(uint32_t (&s)[64], uint64_t see, float scale, float sub, uint32_t t_p) {
+// The 64 weights of a row's half tile from its scores: writes P and returns their sum. An unseen key's
+// score is -inf, its weight 0.
+template <bool kBF16>
+__device__ __forceinline__ float weights(const uint32_t (&s)[64], float scale, float sub, uint32_t t_p) {
   const float2 sc = make_float2(scale, scale), nm = make_float2(-sub, -sub);
   float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint32_t word = static_cast<uint32_t>(see >> (32 * h));
     uint32_t y[16];
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
       const int c = 32 * h + 2 * k;
       const float2 x = ffma2(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc, nm);
-      float p0 = ex2(x.x), p1 = ex2(x.y);
-      if constexpr (kMasked) {
-        p0 = word >> (2 * k) & 1u ? p0 : 0.f;
-        p1 = word >> (2 * k + 1) & 1u ? p1 : 0.f;
-      }
+      const float p0 = ex2(x.x), p1 = ex2(x.y);
       acc[k & 1] = fadd2(acc[k & 1], make_float2(p0, p1));
       y[k] = pack2<kBF16>(p0, p1);
     }
@@ -829,40 +936,41 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const bool has_tail = key_lo + T * 128 > q.ctx;
       float m_run = -INFINITY, l = 0.f;
       uint32_t before = 0, before_phase = 0;  // the previous tile's buffer
-      // One tile, kMasked: some of its keys are nodes, past the length or on a lost page.
-      auto tile = [&](auto masked, int i, bool bad) {
-        constexpr bool kMasked = decltype(masked)::value;
+      for (int i = 0; i < T; ++i) {
         const uint32_t t_s = tmem + lanes + buf * 128 + kb * 64;  // S in, P out
-        uint64_t see = ~0ull;
-        if constexpr (kMasked) {
+        const int key0 = key_lo + i * 128;
+        (void)mbar_wait(&s_full[buf], phase, abort_flag);
+        tc_fence_after_sync();
+        const bool bad = *reinterpret_cast<volatile uint8_t*>(&lost[tiles_done++ % kLostRing]) != 0;
+        const bool masked = bad || key0 + 128 > q.ctx;  // some keys are nodes, past the length or on a lost page
+        uint64_t see = 0ull;
+        if (masked) {
           // S(g) came after PV(g - 3), so V(g)'s barrier is at most this phase behind; P(g) is not
           // released before V(g) is clean, and PV(g) frees V(g)
-          const int key0 = key_lo + i * 128;
           (void)mbar_wait(&v_full[stage], vphase, abort_flag);
           if (key0 + r >= q.ctx) {
             if (clean_v_row<D, kBF16>(sV + stage * C::kTile, r, kb, key0 + r, q)) *reinterpret_cast<volatile int*>(odd_seg) = seg;
             fence_proxy_async_smem();
           }
-          see = live ? seen_bits(p, q, w.b, t, key0 + kb * 64, bad) : 0ull;
+          if (live) see = seen_bits(p, q, w.b, t, key0 + kb * 64, bad);
         }
         if (any_live) {
           uint32_t s[64];
           tmem_ld32(t_s, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
           tmem_ld32(t_s + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
           tmem_wait_ld();
-          float m8[8];
-#pragma unroll
-          for (int u = 0; u < 8; ++u) m8[u] = -INFINITY;
-          if constexpr (kMasked) {
+          if (masked) {
             const uint32_t lo = static_cast<uint32_t>(see), hi = static_cast<uint32_t>(see >> 32);
 #pragma unroll
             for (int c = 0; c < 64; ++c)
-              if ((c < 32 ? lo : hi) >> (c & 31) & 1u) m8[c & 7] = fmaxf(m8[c & 7], __uint_as_float(s[c]));
-          } else {
-#pragma unroll
-            for (int c = 0; c < 64; c += 2)
-              m8[(c >> 1) & 7] = fmax3(m8[(c >> 1) & 7], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+              if (!((c < 32 ? lo : hi) >> (c & 31) & 1u)) s[c] = 0xff800000u;  // -inf
           }
+          float m8[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) m8[u] = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 64; c += 2)
+            m8[(c >> 1) & 7] = fmax3(m8[(c >> 1) & 7], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
           const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
           // two buffers by parity: one is rewritten after the exchange in between
           float* xs = xchg + (xc & 1u) * 256;
@@ -879,7 +987,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             l *= alpha;
           }
           const float sub = m_run == -INFINITY ? 0.f : m_run;  // nothing above -inf so far: weights 0
-          l += weights<kBF16, kMasked>(s, see, p.scale_log2, sub, t_s);
+          l += weights<kBF16>(s, p.scale_log2, sub, t_s);
           if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
             // PV(g - 1) has completed: its barrier's phase before, PV(g - 4), was needed by S(g - 1)
             (void)mbar_wait(&buf_free[before], before_phase, abort_flag);
@@ -909,13 +1017,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           stage = 0;
           vphase ^= 1u;
         }
-      };
-      for (int i = 0; i < T; ++i) {
-        (void)mbar_wait(&s_full[buf], phase, abort_flag);
-        tc_fence_after_sync();
-        const bool bad = *reinterpret_cast<volatile uint8_t*>(&lost[tiles_done++ % kLostRing]) != 0;
-        if (!bad && key_lo + (i + 1) * 128 <= q.ctx) tile(std::false_type{}, i, false);
-        else tile(std::true_type{}, i, bad);
       }
 
       // epilogue: the row's two threads take half the columns each
@@ -1068,8 +1169,26 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
 }
 
 // ------------------------------------------------------------------ host side
+// A launch whose CTAs may start while the kernel before it on the stream still runs; it waits for that
+// kernel's results by griddepcontrol.wait.
+template <typename... Args>
+void launch_after(void (*kernel)(Args...), dim3 grid, int threads, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+inline int simt_rows(int64_t R) { return R <= 16 ? 16 : 32; }
+// Key splits: about four CTAs per SM, none without a tile of the longest row the table allows.
 inline int simt_splits(int64_t units, int64_t tokens) {
-  const int64_t want = (static_cast<int64_t>(current_sm_count()) * 6 + units - 1) / units;
+  const int64_t want = (static_cast<int64_t>(current_sm_count()) * 4 + units - 1) / units;
   return static_cast<int>(std::max<int64_t>(1, std::min({want, (tokens + kKeysTile - 1) / kKeysTile, (int64_t)64})));
 }
 
@@ -1108,10 +1227,11 @@ inline Layout layout(const cab_page_cache* c, int64_t n, int64_t Hq, int64_t T) 
     L.total = L.part_ml + slots * 8;
     return L;
   }
-  L.units = n * c->heads * ((R + kRowsTile - 1) / kRowsTile);
+  const int64_t rows = simt_rows(R);
+  L.units = n * c->heads * ((R + rows - 1) / rows);
   L.splits = simt_splits(L.units, c->width * c->page_size);
   if (L.splits > 1) {
-    const size_t slots = static_cast<size_t>(L.units) * L.splits * kRowsTile;
+    const size_t slots = static_cast<size_t>(L.units) * L.splits * rows;
     L.part_ml = (slots * D * 4 + 15) & ~size_t(15);
     L.total = L.part_ml + slots * 8;
   }
@@ -1150,37 +1270,34 @@ int launch_tc(const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& q
   tc_kernel<D, kBF16><<<L.ctas, kTcThreads, C::kSmem, st>>>(km, vm, qm, p);
   if (int rc = check_launch("tree_attn tc_kernel")) return rc;
   if (L.whole) return CAB_OK;
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(static_cast<unsigned>(L.units), static_cast<unsigned>((L.part_rows + 7) / 8));
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, join_kernel<D, kBF16>, p, L.ctas);
+  launch_after(join_kernel<D, kBF16>, dim3(static_cast<unsigned>(L.units), static_cast<unsigned>((L.part_rows + 7) / 8)), 256, st, p, L.ctas);
   return check_launch("tree_attn join_kernel");
 }
 
-template <typename T, int DC>
+template <typename T, int DC, int RW>
 int launch_simt(const Params& p, int64_t units, cudaStream_t st) {
   const int Dp = (p.D + 3) & ~3;
-  const size_t smem = static_cast<size_t>(kRowsTile * Dp + kKeysTile * (Dp + 4) + kKeysTile * Dp) * 4;
-  if (smem > 48 * 1024) cudaFuncSetAttribute(simt_kernel<T, DC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  simt_kernel<T, DC><<<dim3(static_cast<unsigned>(units), static_cast<unsigned>(p.splits)), kSimtThreads, smem, st>>>(p);
+  const size_t smem = static_cast<size_t>(4 * RW * (Dp + 32) + kKeysTile * (Dp + 4) + kKeysTile * Dp) * 4;
+  if (smem > 48 * 1024) cudaFuncSetAttribute(simt_kernel<T, DC, RW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  simt_kernel<T, DC, RW><<<dim3(static_cast<unsigned>(units), static_cast<unsigned>(p.splits)), kSimtThreads, smem, st>>>(p);
   if (int rc = check_launch("tree_attn simt_kernel")) return rc;
   if (p.splits == 1) return CAB_OK;
-  simt_join_kernel<T, DC><<<static_cast<unsigned>((units * kRowsTile + 3) / 4), kSimtThreads, 0, st>>>(p);
+  launch_after(simt_join_kernel<T, DC>, dim3(static_cast<unsigned>(units * RW)), kSimtThreads, st, p, 4 * RW);
   return check_launch("tree_attn simt_join_kernel");
+}
+
+template <typename T, int DC>
+int launch_simt_rows(const Params& p, int64_t units, cudaStream_t st) {
+  return simt_rows(static_cast<int64_t>(p.G) * p.T) == 16 ? launch_simt<T, DC, 4>(p, units, st) : launch_simt<T, DC, 8>(p, units, st);
 }
 
 template <typename T>
 int launch_simt_d(const Params& p, int64_t units, cudaStream_t st) {
-  if (p.D <= 64) return launch_simt<T, 2>(p, units, st);
-  if (p.D <= 128) return launch_simt<T, 4>(p, units, st);
-  return launch_simt<T, 8>(p, units, st);
+  if (p.D <= 64) return launch_simt_rows<T, 2>(p, units, st);
+  if (p.D <= 128) return launch_simt_rows<T, 4>(p, units, st);
+  return launch_simt_rows<T, 8>(p, units, st);
 }
+
 
 inline int check_sizes(const cab_page_cache* c, int64_t n, int64_t Hq, int64_t T) {
   if (int rc = pages::check_cache(c, "tree_attn", true, false)) return rc;
@@ -1281,6 +1398,10 @@ extern "C" int cab_tree_attn_fwd(const cab_page_cache* cache, int64_t layer, con
       return cache->dim == 128 ? launch_tc<128, true>(km, vm, qm, p, L, st) : launch_tc<64, true>(km, vm, qm, p, L, st);
     return cache->dim == 128 ? launch_tc<128, false>(km, vm, qm, p, L, st) : launch_tc<64, false>(km, vm, qm, p, L, st);
   }
+  // four elements at a time where every row of K and V starts on their size
+  p.in_vec = cache->dim % 4 == 0;
+  for (const void* x : {p.k, p.v}) p.in_vec = p.in_vec && reinterpret_cast<uintptr_t>(x) % (4 * es) == 0;
+  for (int i = 0; i < 3; ++i) p.in_vec = p.in_vec && p.ks[i] % 4 == 0 && p.vs[i] % 4 == 0;
   switch (cache->dtype) {
     case CAB_DTYPE_F32: return launch_simt_d<float>(p, L.units, st);
     case CAB_DTYPE_F16: return launch_simt_d<__half>(p, L.units, st);
