@@ -395,10 +395,14 @@ __global__ void __launch_bounds__(kSimtThreads) simt_join_kernel(const __grid_co
 // fills the GPU; a unit cut between ranges leaves partial sums that join_kernel adds in key order.
 //
 // Tile g of a CTA: S = Q K^T (128 x 128, K-major operands from shared memory) into one of three
-// TMEM buffers; p = 2^(s - m) by two threads per row (64 keys each, which swap their maxima through
-// shared memory), written over S as 16-bit, the products' operand type (its sum is taken before
-// that rounding, in float32); O += P V (P from TMEM, V MN-major as it lies in the pages). S(g + 3) reuses
-// the buffer once PV(g) has completed. O is rescaled only when the maximum has grown by more than 2^8.
+// TMEM buffers; p = 2^(s - m) by one thread per row, written over S as 16-bit, the products' operand
+// type (its sum is taken before that rounding, in float32); O += P V (P from TMEM, V MN-major as it lies in
+// the pages). S(g + 3) reuses the buffer once PV(g) has completed. Two sets of four warps take turns,
+// one tile each: a set takes its tile's maxima, gets the rows' reference m from the other set's tile
+// before, passes m on and then computes the weights, so that on each SM quarter one warp's exponentials
+// (the special function unit's 1024 clocks a tile, as many as the products take) run under the other's
+// loads and maxima. (Both sets on one tile, half the keys each, wait for one another: 2050 clocks a tile.)
+// m, and with it O, changes only when a maximum exceeds it by more than 2^8.
 //
 // Warps 0 and 3 look up the pages and load K and V by TMA (one box per page and 64 columns, a lane
 // each; a page number outside the pool reads zeros), so loads are issued from two warps (one warp
@@ -426,8 +430,8 @@ struct Cfg {
   static constexpr int kStages = D == 128 ? 3 : 6;  // of K, and of V
   // with as many stages as S / P buffers S(g) completed frees K stage g % 3, PV(g) V stage g % 3
   static constexpr bool kOneSignal = kStages == kBufs;
-  static constexpr int kXchg = 2 * 2 * 128 * 4;  // row maxima / sums [parity][key half][row]
-  static constexpr int kBars = (4 * kStages + 3 * kBufs + 3) * 8 + 32 + kLostRing;
+  static constexpr int kXchg = 2 * 2 * 128 * 4;  // references m [tile parity][row], sums [set][row]
+  static constexpr int kBars = (4 * kStages + 3 * kBufs + 4) * 8 + 32 + kLostRing;
   static constexpr int kBytes = (1 + 2 * kStages) * kTile + kXchg + kBars;
   static constexpr int kSmem = kBytes + 1024 < 232448 ? kBytes + 1024 : 232448;  // the kernel checks that it fits
   static_assert(kBytes <= 232448, "shared memory");
@@ -545,7 +549,7 @@ __device__ __forceinline__ Begin find_range(const Params& p, const Share& sh, in
 __device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
 // Which of the keys key0 .. key0 + 63 node t of sequence b sees.
-__device__ __forceinline__ uint64_t seen_bits(const Params& p, const Seq& s, int b, int t, int key0, bool bad_pages) {
+__device__ __noinline__ uint64_t seen_bits(const Params& p, const Seq& s, int b, int t, int key0, bool bad_pages) {
   const int c = s.ctx - key0;
   uint64_t w = low_bits(c);
   if (p.parents) {
@@ -590,34 +594,33 @@ __device__ __forceinline__ void fix_up(const Params& p, const Seq& s, int b, int
   }
 }
 
-// Half `half` (D / 2 columns) of row r of a V tile: past the length it becomes 0; of a node, elements
-// that are not finite do. Returns whether there were any.
+// Row r of a V tile: past the length it becomes 0; of a node, elements that are not finite do. Returns
+// whether there were any.
 template <int D, bool kBF16>
-__device__ __forceinline__ bool clean_v_row(uint8_t* tile, int r, int half, int key, const Seq& s) {
+__device__ __forceinline__ bool clean_v_row(uint8_t* tile, int r, int key, const Seq& s) {
   constexpr uint32_t kExp = kBF16 ? 0x7F807F80u : 0x7C007C00u, kOne = kBF16 ? 0x00800080u : 0x04000400u;
-  const int x0 = half * (D / 16);  // first 16-byte chunk of the row
   auto chunk = [&](int x) { return reinterpret_cast<uint4*>(tile + (x >> 3) * 16384 + sw128_offset(r, x & 7)); };
   if (key >= s.len) {
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) *chunk(x0 + c) = make_uint4(0, 0, 0, 0);
+    for (int c = 0; c < D / 8; ++c) *chunk(c) = make_uint4(0, 0, 0, 0);
     return false;
   }
   uint32_t hit = 0u;  // an exponent of ones carries into the bit above it
 #pragma unroll
-  for (int c = 0; c < D / 16; ++c) {
-    const uint4 v = *chunk(x0 + c);
+  for (int c = 0; c < D / 8; ++c) {
+    const uint4 v = *chunk(c);
     hit |= ((v.x & kExp) + kOne) | ((v.y & kExp) + kOne) | ((v.z & kExp) + kOne) | ((v.w & kExp) + kOne);
   }
   if ((hit & 0x80008000u) == 0u) return false;
-  for (int c = 0; c < D / 16; ++c) {
-    uint4 v = *chunk(x0 + c);
+  for (int c = 0; c < D / 8; ++c) {
+    uint4 v = *chunk(c);
     uint32_t* e = reinterpret_cast<uint32_t*>(&v);
     for (int k = 0; k < 4; ++k) {
       const uint32_t h = ((e[k] & kExp) + kOne) & 0x80008000u;
       if (h & 0x8000u) e[k] &= 0xFFFF0000u;
       if (h & 0x80000000u) e[k] &= 0x0000FFFFu;
     }
-    *chunk(x0 + c) = v;
+    *chunk(c) = v;
   }
   return true;
 }
@@ -636,7 +639,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 __device__ __forceinline__ void softmax_sync() {  // the 256 threads of the softmax warps
   asm volatile("barrier.cta.sync 5, 256;" ::: "memory");
 }
+// The two warps of a row quarter: a meeting of both, and a handing on from the warp of one tile to that
+// of the next (barriers by the parity of the tile).
 __device__ __forceinline__ void pair_sync(int quad) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(1 + quad) : "memory"); }
+__device__ __forceinline__ void hand_on(int quad, int parity) {
+  asm volatile("barrier.cta.arrive %0, 64;" ::"r"(6 + 2 * quad + parity) : "memory");
+}
+__device__ __forceinline__ void take_over(int quad, int parity) {
+  asm volatile("barrier.cta.sync %0, 64;" ::"r"(6 + 2 * quad + parity) : "memory");
+}
 
 __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -704,10 +715,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* k_empty = v_full + kStages;    // unused with kOneSignal
   uint64_t* v_empty = k_empty + kStages;   // unused with kOneSignal
   uint64_t* s_full = v_empty + kStages;    // [3] S(g) is there
-  uint64_t* p_full = s_full + kBufs;       // [3] P(g) is there (8 warps)
+  uint64_t* p_full = s_full + kBufs;       // [3] P(g) is there (4 warps)
   uint64_t* buf_free = p_full + kBufs;     // [3] PV(g) has completed
   uint64_t* q_full = buf_free + kBufs;     // Q of the segment is there
-  uint64_t* drain = q_full + 1;            // [2]
+  uint64_t* q_free = q_full + 1;           // the segment's products with Q have completed
+  uint64_t* drain = q_free + 1;            // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   int* odd_seg = abort_flag + 1;   // the last segment (from 1) whose V tiles held values that are not finite
@@ -733,10 +745,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int s = 0; s < 4 * kStages; ++s) mbar_init(&k_full[s], 1);
     for (int s = 0; s < kBufs; ++s) {
       mbar_init(&s_full[s], 2);  // the product, and the issuer itself: it passes on what the K loader wrote
-      mbar_init(&p_full[s], 8);
+      mbar_init(&p_full[s], 4);
       mbar_init(&buf_free[s], 1);
     }
     mbar_init(q_full, 1);
+    mbar_init(q_free, 1);
     mbar_init(&drain[0], 1);
     mbar_init(&drain[1], 1);
     *abort_flag = 0;
@@ -804,7 +817,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (is_k) {
         // Q, once the previous segment's last S, its reader, has completed (S runs ahead of the
         // softmax, so the next segment's first S is done by the time the softmax gets there)
-        if (g > 0) ok = mbar_wait(&s_full[(g - 1) % kBufs], ((g - 1) / kBufs) & 1, abort_flag);
+        if (nq > 0) ok = mbar_wait(q_free, (nq - 1) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ++nq;
@@ -874,6 +887,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           mma_commit(&s_full[buf]);
           mbar_arrive(&s_full[buf]);
         }
+        mma_commit(q_free);
       }
       mma_commit(&drain[0]);
       (void)mbar_wait(&drain[0], 0, nullptr);
@@ -890,8 +904,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int T = segment_of(p, sh, w, w.set * sh.wide + side).count;
         for (int i = 0; i < T; ++i, ++g) {
           const uint32_t st = g % kStages, buf = g % kBufs;
-          // V normally lands early; P(g) is the event waited on last. All warps have read the
-          // previous segment's O before they release its first P.
+          // V normally lands early; P(g) is the event waited on last. The previous segment's O has been
+          // read before the first P is released.
           if (!mbar_wait(&v_full[st], (g / kStages) & 1, abort_flag) ||
               !mbar_wait(&p_full[buf], (g / kBufs) & 1, abort_flag)) {
             ok = false;
@@ -901,7 +915,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const uint64_t dv = dV + static_cast<uint64_t>((st * C::kTile) >> 4);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            mma_f16_ts(tmem + kTmemO, tmem + buf * 128 + (kk >> 2) * 64 + (kk & 3) * 8,
+            mma_f16_ts(tmem + kTmemO, tmem + buf * 128 + kk * 8,
                        dv + static_cast<uint64_t>(kk * (2048 >> 4)), idesc, (i > 0 || kk > 0) ? 1u : 0u);
           if constexpr (!C::kOneSignal) mma_commit(&v_empty[st]);
           mma_commit(&buf_free[buf]);
@@ -913,14 +927,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax and epilogue
-    // Warp w owns TMEM lanes 32 * (w & 3) .. + 31 (rows) and key half kb = (w - 4) / 4 of every tile.
+    // Warp w owns TMEM lanes 32 * (w & 3) .. + 31 (rows); set kb = (w - 4) / 4 takes every other tile.
     // A wait that gave up does not end the loops: the barriers stay matched, and every later wait
     // returns at once.
     const int quad = warp & 3, kb = (warp - 4) >> 2, r = quad * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t t_o = tmem + lanes + kTmemO + kb * (D / 2);
-    // tile g's S / P buffer and barrier phase, and its V stage and phase, counted instead of divided
-    uint32_t buf = 0, phase = 0, stage = 0, vphase = 0, xc = 0, tiles_done = 0;
+    const uint32_t t_o = tmem + lanes + kTmemO;
+    float *ref = xchg, *sums = xchg + 256;
+    uint32_t g0 = 0;  // tiles of earlier segments
     int seg = 0;
     for (; w.left > 0; walk_next(p, sh, w)) {
       const int grp = w.set * sh.wide + side;
@@ -934,66 +948,80 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const bool any_live = __any_sync(0xffffffffu, live);
       const int key_lo = sg.first * 128, keys = group_keys(p, sh, q, grp, grp);
       const bool has_tail = key_lo + T * 128 > q.ctx;
-      float m_run = -INFINITY, l = 0.f;
-      uint32_t before = 0, before_phase = 0;  // the previous tile's buffer
-      for (int i = 0; i < T; ++i) {
-        const uint32_t t_s = tmem + lanes + buf * 128 + kb * 64;  // S in, P out
+      float m_run = -INFINITY, l = 0.f;  // this set's sum, relative to its last m
+      for (int i = kb; i < T; i += 2) {
+        const uint32_t g = g0 + i, buf = g % kBufs;
+        const uint32_t t_s = tmem + lanes + buf * 128;  // S in, P out
         const int key0 = key_lo + i * 128;
-        (void)mbar_wait(&s_full[buf], phase, abort_flag);
+        // tiles between this set's were S before this one, so the barrier is at most this phase behind
+        (void)mbar_wait(&s_full[buf], (g / kBufs) & 1, abort_flag);
         tc_fence_after_sync();
-        const bool bad = *reinterpret_cast<volatile uint8_t*>(&lost[tiles_done++ % kLostRing]) != 0;
+        const bool bad = *reinterpret_cast<volatile uint8_t*>(&lost[g % kLostRing]) != 0;
         const bool masked = bad || key0 + 128 > q.ctx;  // some keys are nodes, past the length or on a lost page
-        uint64_t see = 0ull;
+        uint64_t see[2] = {0ull, 0ull};
         if (masked) {
           // S(g) came after PV(g - 3), so V(g)'s barrier is at most this phase behind; P(g) is not
           // released before V(g) is clean, and PV(g) frees V(g)
-          (void)mbar_wait(&v_full[stage], vphase, abort_flag);
+          const uint32_t st = g % kStages;
+          (void)mbar_wait(&v_full[st], (g / kStages) & 1, abort_flag);
           if (key0 + r >= q.ctx) {
-            if (clean_v_row<D, kBF16>(sV + stage * C::kTile, r, kb, key0 + r, q)) *reinterpret_cast<volatile int*>(odd_seg) = seg;
+            if (clean_v_row<D, kBF16>(sV + st * C::kTile, r, key0 + r, q)) *reinterpret_cast<volatile int*>(odd_seg) = seg;
             fence_proxy_async_smem();
           }
-          if (live) see = seen_bits(p, q, w.b, t, key0 + kb * 64, bad);
+          if (live) {
+            see[0] = seen_bits(p, q, w.b, t, key0, bad);
+            see[1] = seen_bits(p, q, w.b, t, key0 + 64, bad);
+          }
         }
         if (any_live) {
           uint32_t s[64];
-          tmem_ld32(t_s, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-          tmem_ld32(t_s + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
-          tmem_wait_ld();
-          if (masked) {
-            const uint32_t lo = static_cast<uint32_t>(see), hi = static_cast<uint32_t>(see >> 32);
+          auto load_half = [&](int h) {
+            tmem_ld32(t_s + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+            tmem_ld32(t_s + 64 * h + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+            tmem_wait_ld();
+            if (masked) {
+              const uint32_t lo = static_cast<uint32_t>(see[h]), hi = static_cast<uint32_t>(see[h] >> 32);
 #pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (!((c < 32 ? lo : hi) >> (c & 31) & 1u)) s[c] = 0xff800000u;  // -inf
-          }
+              for (int c = 0; c < 64; ++c)
+                if (!((c < 32 ? lo : hi) >> (c & 31) & 1u)) s[c] = 0xff800000u;  // -inf
+            }
+          };
           float m8[8];
 #pragma unroll
           for (int u = 0; u < 8; ++u) m8[u] = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < 64; c += 2)
-            m8[(c >> 1) & 7] = fmax3(m8[(c >> 1) & 7], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-          const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
-          // two buffers by parity: one is rewritten after the exchange in between
-          float* xs = xchg + (xc & 1u) * 256;
-          xs[kb * 128 + r] = mx;
-          pair_sync(quad);
-          ++xc;
-          const float m_tile = fmaxf(mx, xs[(kb ^ 1) * 128 + r]) * p.scale_log2;
-          float alpha = 1.f;
-          if (m_run == -INFINITY) {
-            m_run = m_tile;
-          } else if (m_tile > m_run + kRescaleThreshold) {
-            alpha = ex2(m_run - m_tile);
-            m_run = m_tile;
-            l *= alpha;
-          }
-          const float sub = m_run == -INFINITY ? 0.f : m_run;  // nothing above -inf so far: weights 0
-          l += weights<kBF16>(s, p.scale_log2, sub, t_s);
-          if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-            // PV(g - 1) has completed: its barrier's phase before, PV(g - 4), was needed by S(g - 1)
-            (void)mbar_wait(&buf_free[before], before_phase, abort_flag);
-            tc_fence_after_sync();
+          for (int h = 1; h >= 0; --h) {  // the first half last: its scores are in registers for the weights
+            load_half(h);
 #pragma unroll
-            for (int c = 0; c < D / 2; c += 32) {
+            for (int c = 0; c < 64; c += 2)
+              m8[(c >> 1) & 7] = fmax3(m8[(c >> 1) & 7], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+          }
+          const float m_tile = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) *
+                               p.scale_log2;
+          float m_prev = -INFINITY;
+          if (i > 0) {
+            take_over(quad, (i - 1) & 1);
+            m_prev = ref[((i - 1) & 1) * 128 + r];
+          }
+          const float m_new = m_prev == -INFINITY || m_tile > m_prev + kRescaleThreshold ? m_tile : m_prev;
+          if (i + 1 < T) {
+            ref[(i & 1) * 128 + r] = m_new;
+            hand_on(quad, i & 1);
+          }
+          if (m_run != m_new) l *= ex2(m_run - m_new);  // from -inf: l is 0
+          m_run = m_new;
+          const float sub = m_new == -INFINITY ? 0.f : m_new;  // nothing above -inf so far: weights 0
+          l += weights<kBF16>(s, p.scale_log2, sub, t_s);
+          load_half(1);
+          l += weights<kBF16>(s, p.scale_log2, sub, t_s + 32);
+          const bool grown = m_prev != -INFINITY && m_new != m_prev;
+          if (__any_sync(0xffffffffu, grown)) {
+            // PV(g - 1) has completed: its barrier's phase before, PV(g - 4), was needed by S(g - 1)
+            (void)mbar_wait(&buf_free[(g - 1) % kBufs], ((g - 1) / kBufs) & 1, abort_flag);
+            tc_fence_after_sync();
+            const float alpha = grown ? ex2(m_prev - m_new) : 1.f;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
               uint32_t x[32];
               tmem_ld32(t_o + c, x);
               tmem_wait_ld();
@@ -1007,27 +1035,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[buf]);
-        before = buf;
-        before_phase = phase;
-        if (++buf == kBufs) {
-          buf = 0;
-          phase ^= 1u;
-        }
-        if (++stage == kStages) {
-          stage = 0;
-          vphase ^= 1u;
-        }
       }
+      g0 += T;
 
       // epilogue: the row's two threads take half the columns each
-      (void)mbar_wait(&buf_free[before], before_phase, abort_flag);
-      tc_fence_after_sync();
       if (any_live) {
-        float* xs = xchg + (xc & 1u) * 256;
-        xs[kb * 128 + r] = l;
+        const int last = (T - 1) & 1;
+        if (kb == last) ref[last * 128 + r] = m_run;
         pair_sync(quad);
-        ++xc;
-        l += xs[(kb ^ 1) * 128 + r];
+        const float m_end = ref[last * 128 + r];
+        if (m_run != m_end) l *= ex2(m_run - m_end);
+        m_run = m_end;
+        sums[kb * 128 + r] = l;
+        pair_sync(quad);
+        l += sums[(kb ^ 1) * 128 + r];
+        // the last tile's S was seen by one of the pair, so its PV's barrier is at most this phase behind
+        (void)mbar_wait(&buf_free[(g0 - 1) % kBufs], ((g0 - 1) / kBufs) & 1, abort_flag);
+        tc_fence_after_sync();
       }
       if (has_tail) softmax_sync();  // all warps have cleaned their part of V
       if (quad * 32 < rows) {
@@ -1042,7 +1066,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int c = 0; c < D / 2; c += 32) {
           uint32_t x[32];
           if (any_live) {
-            tmem_ld32(t_o + c, x);
+            tmem_ld32(t_o + kb * (D / 2) + c, x);
             tmem_wait_ld();
           }
           if (r >= rows) continue;
@@ -1089,6 +1113,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       tc_fence_before_sync();
+      if (any_live) pair_sync(quad);  // both have read O: the next segment's products may overwrite it
     }
   }
   __syncthreads();
