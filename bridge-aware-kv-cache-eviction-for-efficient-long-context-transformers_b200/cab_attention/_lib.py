@@ -7,6 +7,7 @@ library is missing or the tensors are not on an sm_100 CUDA device, the call rai
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 from pathlib import Path
@@ -133,6 +134,12 @@ def ptr(t) -> int | None:
 
 def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+@functools.lru_cache(maxsize=1024)
+def strides(a: int, b: int, c: int):
+    """Three strides as the C ABI takes them (made once for each triple)."""
+    return _i64_3(a, b, c)
 
 
 def raw_stream(index: int) -> int:

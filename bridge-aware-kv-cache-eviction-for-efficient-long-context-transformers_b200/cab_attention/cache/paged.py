@@ -180,7 +180,7 @@ class PagedKVCache:
         if v.stride(3) != 1:
             v = v.contiguous()
         call_on(self.device, "cab_pages_write", _lib.lib().cab_pages_write, self._c, layer, k.data_ptr(), v.data_ptr(),
-                n, T, _lib.strides3(k), _lib.strides3(v), _lib.ptr(rows), _lib.ptr(num_new), T)
+                n, T, _lib.strides(*k.stride()[:3]), _lib.strides(*v.stride()[:3]), _lib.ptr(rows), _lib.ptr(num_new), T)
 
     def attend(self, layer: int, q: torch.Tensor, parents: Optional[torch.Tensor] = None,
                tree_mask: Optional[torch.Tensor] = None, num_nodes: Optional[torch.Tensor] = None,

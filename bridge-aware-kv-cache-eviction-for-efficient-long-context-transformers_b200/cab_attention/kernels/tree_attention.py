@@ -141,8 +141,7 @@ def attend_cache(cache, device, dtype, layer: int, q: torch.Tensor, parents=None
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     os = out.stride()
     call_on(device, "cab_tree_attn_fwd", L.cab_tree_attn_fwd, cache, layer, q.data_ptr(), out.data_ptr(),
-            None if lse is None else lse.data_ptr(), n, Hq, T, _lib._i64_3(qs[0], qs[1], qs[2]),
-            _lib._i64_3(os[0], os[1], os[2]), _lib.ptr(rows), _lib.ptr(num_nodes), _lib.ptr(parents), parents_stride,
+            None if lse is None else lse.data_ptr(), n, Hq, T, _lib.strides(*qs[:3]), _lib.strides(*os[:3]), _lib.ptr(rows), _lib.ptr(num_nodes), _lib.ptr(parents), parents_stride,
             _lib.ptr(tree_mask), mask_stride, scale, None if ws is None else ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 

@@ -522,14 +522,19 @@ struct Begin {
 };
 __device__ __forceinline__ Begin find_range(const Params& p, const Share& sh, int range, int most) {
   const int lane = threadIdx.x & 31;
-  const int64_t total = total_weight(p, sh);
+  int64_t own = 0;  // up to 32 sequences: one reading for the total and the place
+  if (p.n <= 32 && lane < p.n) own = static_cast<int64_t>(head_weight(p, sh, load_seq(p, lane))) * p.Hkv;
+  int64_t total = own;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (p.n > 32) total = total_weight(p, sh);
   const int ranges = range_count(total, most, p.least);
   if (range >= ranges) return Begin{0, 0, 0};
   const int64_t f0 = range_start(total, ranges, range), f1 = range_start(total, ranges, range + 1);
   int64_t base = 0;
   for (int b0 = 0; b0 < p.n; b0 += 32) {
-    const int b = b0 + lane;  // the second reading of the lengths hits L1
-    const int64_t own = b < p.n ? static_cast<int64_t>(head_weight(p, sh, load_seq(p, b))) * p.Hkv : 0;
+    const int b = b0 + lane;
+    if (p.n > 32) own = b < p.n ? static_cast<int64_t>(head_weight(p, sh, load_seq(p, b))) * p.Hkv : 0;  // L1
     int64_t inc = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -548,31 +553,50 @@ __device__ __forceinline__ Begin find_range(const Params& p, const Share& sh, in
 
 __device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
-// Which of the keys key0 .. key0 + 63 node t of sequence b sees.
-__device__ __noinline__ uint64_t seen_bits(const Params& p, const Seq& s, int b, int t, int key0, bool bad_pages) {
+struct Bits {
+  uint64_t lo, hi;
+};
+
+// Which of the keys key0 .. key0 + 127 node t of sequence b sees.
+__device__ __forceinline__ Bits seen_bits(const Params& p, const Seq& s, int b, int t, int key0, bool bad_pages) {
   const int c = s.ctx - key0;
-  uint64_t w = low_bits(c);
+  Bits w{low_bits(c), low_bits(c - 64)};
   if (p.parents) {
     const int32_t* up = p.parents + b * p.parents_stride;
     for (int x = t; x >= 0;) {
-      const int at = c + x;
+      const int y = up[x], at = c + x;
       if (at < 0) break;
-      if (at < 64) w |= 1ull << at;
-      const int y = up[x];
+      if (at < 64) w.lo |= 1ull << at;
+      else if (at < 128) w.hi |= 1ull << (at - 64);
       if (y >= x) break;
       x = y;
     }
   } else if (p.mask) {
-    const uint8_t* row = p.mask + b * p.mask_stride + static_cast<int64_t>(t) * p.T;
-    for (int at = max(c, 0); at < min(64, c + s.m); ++at)
-      if (row[at - c]) w |= 1ull << at;
+    const uint8_t* row = p.mask + b * p.mask_stride + static_cast<int64_t>(t) * p.T - c;
+    const int end = min(128, c + s.m);
+#pragma unroll 1
+    for (int at0 = max(c, 0); at0 < end; at0 += 16) {
+      uint32_t v[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) v[u] = at0 + u < end ? row[at0 + u] : 0u;
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        const uint64_t bit = v[u] != 0u ? 1ull << ((at0 + u) & 63) : 0ull;
+        if (at0 + u < 64) w.lo |= bit;
+        else w.hi |= bit;
+      }
+    }
   } else {
-    w = low_bits(c + t + 1);
+    w.lo = low_bits(c + t + 1);
+    w.hi = low_bits(c + t + 1 - 64);
   }
   if (bad_pages) {
-    for (int j = 0; j < 64 && key0 + j < s.len; ++j) {
+    for (int j = 0; j < 128 && key0 + j < s.len; ++j) {
       const int pg = p.table[s.row * p.table_stride + (key0 + j) / p.page_size];
-      if (pg < 0 || pg >= p.pages) w &= ~(1ull << j);
+      if (pg < 0 || pg >= p.pages) {
+        if (j < 64) w.lo &= ~(1ull << j);
+        else w.hi &= ~(1ull << (j - 64));
+      }
     }
   }
   return w;
@@ -738,10 +762,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int range = blockIdx.x / sh.wide, side = blockIdx.x % sh.wide;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (threadIdx.x == 32) {
-    prefetch_tensormap(&kmap);
-    prefetch_tensormap(&vmap);
-    prefetch_tensormap(&qmap);
+  if (threadIdx.x == 0) {
     for (int s = 0; s < 4 * kStages; ++s) mbar_init(&k_full[s], 1);
     for (int s = 0; s < kBufs; ++s) {
       mbar_init(&s_full[s], 2);  // the product, and the issuer itself: it passes on what the K loader wrote
@@ -756,19 +777,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     *odd_seg = 0;
     fence_barrier_init();
   }
+  if (threadIdx.x == 32) {
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&vmap);
+    prefetch_tensormap(&qmap);
+  }
   if (warp == 2) tmem_alloc(tmem_slot, 512);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the inputs of this call may be the kernel before's results
   if (warp == 0) {
+    __syncwarp();
     const Begin x = find_range(p, sh, range, gridDim.x / sh.wide);
     if (lane == 0) {
       begin[0] = x.b;
       begin[1] = x.offset;
       begin[2] = x.left;
     }
+    __syncwarp();
   }
   tc_fence_before_sync();
-  __syncthreads();
+  if (warp == 0) asm volatile("barrier.cta.arrive 14, %0;" ::"n"(kTcThreads) : "memory");  // K needs nobody else
+  else asm volatile("barrier.cta.sync 14, %0;" ::"n"(kTcThreads) : "memory");
   tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = warp == 0 ? 0u : *tmem_slot;
 
   Walk w;
   w.b = begin[0];
@@ -958,8 +988,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_after_sync();
         const bool bad = *reinterpret_cast<volatile uint8_t*>(&lost[g % kLostRing]) != 0;
         const bool masked = bad || key0 + 128 > q.ctx;  // some keys are nodes, past the length or on a lost page
-        uint64_t see[2] = {0ull, 0ull};
+        Bits see{~0ull, ~0ull};
         if (masked) {
+          see = Bits{0ull, 0ull};
           // S(g) came after PV(g - 3), so V(g)'s barrier is at most this phase behind; P(g) is not
           // released before V(g) is clean, and PV(g) frees V(g)
           const uint32_t st = g % kStages;
@@ -968,10 +999,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (clean_v_row<D, kBF16>(sV + st * C::kTile, r, key0 + r, q)) *reinterpret_cast<volatile int*>(odd_seg) = seg;
             fence_proxy_async_smem();
           }
-          if (live) {
-            see[0] = seen_bits(p, q, w.b, t, key0, bad);
-            see[1] = seen_bits(p, q, w.b, t, key0 + 64, bad);
-          }
+          if (live) see = seen_bits(p, q, w.b, t, key0, bad);
         }
         if (any_live) {
           uint32_t s[64];
@@ -979,8 +1007,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tmem_ld32(t_s + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
             tmem_ld32(t_s + 64 * h + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
             tmem_wait_ld();
-            if (masked) {
-              const uint32_t lo = static_cast<uint32_t>(see[h]), hi = static_cast<uint32_t>(see[h] >> 32);
+            const uint64_t word = h ? see.hi : see.lo;
+            if (__any_sync(0xffffffffu, word != ~0ull)) {  // else all of the warp's rows see the whole half
+              const uint32_t lo = static_cast<uint32_t>(word), hi = static_cast<uint32_t>(word >> 32);
 #pragma unroll
               for (int c = 0; c < 64; ++c)
                 if (!((c < 32 ? lo : hi) >> (c & 31) & 1u)) s[c] = 0xff800000u;  // -inf
@@ -1197,11 +1226,12 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
 // A launch whose CTAs may start while the kernel before it on the stream still runs; it waits for that
 // kernel's results by griddepcontrol.wait.
 template <typename... Args>
-void launch_after(void (*kernel)(Args...), dim3 grid, int threads, cudaStream_t st, Args... args) {
+void launch_after(void (*kernel)(Args...), dim3 grid, int threads, cudaStream_t st, int smem, Args... args) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1292,10 +1322,10 @@ int launch_tc(const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& q
     cudaFuncSetAttribute(tc_kernel<D, kBF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (dev >= 0 && dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  tc_kernel<D, kBF16><<<L.ctas, kTcThreads, C::kSmem, st>>>(km, vm, qm, p);
+  launch_after(tc_kernel<D, kBF16>, dim3(L.ctas), kTcThreads, st, C::kSmem, km, vm, qm, p);
   if (int rc = check_launch("tree_attn tc_kernel")) return rc;
   if (L.whole) return CAB_OK;
-  launch_after(join_kernel<D, kBF16>, dim3(static_cast<unsigned>(L.units), static_cast<unsigned>((L.part_rows + 7) / 8)), 256, st, p, L.ctas);
+  launch_after(join_kernel<D, kBF16>, dim3(static_cast<unsigned>(L.units), static_cast<unsigned>((L.part_rows + 7) / 8)), 256, st, 0, p, L.ctas);
   return check_launch("tree_attn join_kernel");
 }
 
@@ -1307,7 +1337,7 @@ int launch_simt(const Params& p, int64_t units, cudaStream_t st) {
   simt_kernel<T, DC, RW><<<dim3(static_cast<unsigned>(units), static_cast<unsigned>(p.splits)), kSimtThreads, smem, st>>>(p);
   if (int rc = check_launch("tree_attn simt_kernel")) return rc;
   if (p.splits == 1) return CAB_OK;
-  launch_after(simt_join_kernel<T, DC>, dim3(static_cast<unsigned>(units * RW)), kSimtThreads, st, p, 4 * RW);
+  launch_after(simt_join_kernel<T, DC>, dim3(static_cast<unsigned>(units * RW)), kSimtThreads, st, 0, p, 4 * RW);
   return check_launch("tree_attn simt_join_kernel");
 }
 
