@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
   uint32_t* b_dst = reinterpret_cast<uint32_t*>(sh + 15 * n + 1);
   uint32_t *b_src = b_dst + words, *b_multi = b_src + words;
   grid_launch_dependents();
+  grid_dependency_wait();  // the kernel before may have written the state or this call's lists
 
   // pass 0: the pairs and their checks (the same in every CTA)
   int err = *reinterpret_cast<volatile int32_t*>(c.status) != 0 ? kFrozen : 0;
@@ -503,6 +504,7 @@ struct WriteParams {
 template <typename V>
 __global__ void __launch_bounds__(256) write_kernel(const __grid_constant__ WriteParams p, int vec_elems, int vecs) {
   const cab_page_cache& c = p.c;
+  grid_dependency_wait();
   if (*reinterpret_cast<volatile int32_t*>(c.status) != 0) return;
   const int64_t S = c.page_size;
   const int64_t groups = (p.T + 31) / 32, tasks = groups * c.heads * p.n;
@@ -547,6 +549,26 @@ __global__ void __launch_bounds__(256) write_kernel(const __grid_constant__ Writ
 }
 
 // ------------------------------------------------------------------ host side
+// A launch whose CTAs may start while the kernel before it on the stream still runs; it waits for that
+// kernel's results by griddepcontrol.wait. `cluster` CTAs form a cluster.
+template <typename... Args>
+void launch_after(void (*kernel)(Args...), dim3 grid, int threads, cudaStream_t st, size_t smem, int cluster, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 inline int check_cache(const cab_page_cache* c, const char* what, bool data, bool state = true) {
   if (!c) return fail(CAB_ERR_INVALID_ARG, "%s: NULL cache", what);
   if (!c->block_table || !c->seq_lens || (state && (!c->ref_counts || !c->status)))
@@ -666,18 +688,8 @@ extern "C" int cab_pages_update(const cab_page_cache* cache, const int32_t* src,
     cudaFuncSetAttribute(update_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   // one CTA reads up to 8 values a thread of each array in one go; more are spread over a cluster
   const int64_t ints = std::max(cache->pages, n * std::max(cache->width, keep_cols));
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(ints > 8 * kUpdateThreads ? kMaxCluster : 1);
-  cfg.blockDim = dim3(kUpdateThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cfg.gridDim.x;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, update_kernel, p);
+  launch_after(update_kernel, dim3(ints > 8 * kUpdateThreads ? kMaxCluster : 1), kUpdateThreads, static_cast<cudaStream_t>(stream), smem,
+               ints > 8 * kUpdateThreads ? kMaxCluster : 1, p);
   if (int rc = check_launch("pages update_kernel")) return rc;
   if (!copies) return CAB_OK;
 
@@ -687,18 +699,11 @@ extern "C" int cab_pages_update(const cab_page_cache* cache, const int32_t* src,
   // without a list only a pair's last page is copied, else at most keep_cols + page_size tokens
   const int64_t per = keep_cols > 0 ? (keep_cols + cache->page_size - 1) / cache->page_size + 1 : 1;
   const int64_t most = std::min(L.cap, n * std::min(per, cache->width)) * ((cache->page_size + 31) / 32) * cache->layers * cache->heads;
-  cudaLaunchConfig_t cc{};
-  cudaLaunchAttribute ca[1];
-  cc.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((most + 7) / 8, (int64_t)current_sm_count() * 8))));
-  cc.blockDim = dim3(256);
-  cc.stream = static_cast<cudaStream_t>(stream);
-  ca[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  ca[0].val.programmaticStreamSerializationAllowed = 1;
-  cc.attrs = ca;
-  cc.numAttrs = 1;
-  if (vb == 16) cudaLaunchKernelEx(&cc, copy_kernel<uint4>, p, ve, vecs);
-  else if (vb == 4) cudaLaunchKernelEx(&cc, copy_kernel<uint32_t>, p, ve, vecs);
-  else cudaLaunchKernelEx(&cc, copy_kernel<uint16_t>, p, ve, vecs);
+  const dim3 grid(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((most + 7) / 8, (int64_t)current_sm_count() * 8))));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (vb == 16) launch_after(copy_kernel<uint4>, grid, 256, st, 0, 1, p, ve, vecs);
+  else if (vb == 4) launch_after(copy_kernel<uint32_t>, grid, 256, st, 0, 1, p, ve, vecs);
+  else launch_after(copy_kernel<uint16_t>, grid, 256, st, 0, 1, p, ve, vecs);
   return check_launch("pages copy_kernel");
 }
 
@@ -736,8 +741,8 @@ extern "C" int cab_pages_write(const cab_page_cache* cache, int64_t layer, const
   const int64_t tasks = (T + 31) / 32 * cache->heads * n;
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>((tasks + 7) / 8, (int64_t)current_sm_count() * 8));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (vb == 16) write_kernel<uint4><<<grid, 256, 0, st>>>(p, ve, vecs);
-  else if (vb == 4) write_kernel<uint32_t><<<grid, 256, 0, st>>>(p, ve, vecs);
-  else write_kernel<uint16_t><<<grid, 256, 0, st>>>(p, ve, vecs);
+  if (vb == 16) launch_after(write_kernel<uint4>, dim3(grid), 256, st, 0, 1, p, ve, vecs);
+  else if (vb == 4) launch_after(write_kernel<uint32_t>, dim3(grid), 256, st, 0, 1, p, ve, vecs);
+  else launch_after(write_kernel<uint16_t>, dim3(grid), 256, st, 0, 1, p, ve, vecs);
   return check_launch("pages write_kernel");
 }
