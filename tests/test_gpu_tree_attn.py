@@ -142,6 +142,81 @@ def test_matches_oracle(Hq, H, D, S, T, ctx, tree, dtype):
     check(out, lse, q, ks, vs, nodes, 1 / math.sqrt(D), dtype, parents, mask)
 
 
+# shapes of the scheduling: many sequences, heads that fill a tile or exceed it, long rows cut between
+# CTAs, short rows in wide tables, large pages
+SHAPES = [
+    # Hq, Hkv, D, S, T, ctx, width (pages of a table row, 0: as needed), dtype
+    (4, 2, 64, 16, 2, [37 * i % 400 for i in range(40)], 0, BF),
+    (2, 2, 128, 16, 1, [11 * i % 90 for i in range(150)], 0, HF),
+    (2, 1, 64, 64, 3, [5 + 7 * i for i in range(33)], 2048, BF),
+    (128, 1, 128, 32, 3, [700, 20], 0, BF),     # a node fills a tile
+    (130, 1, 64, 16, 2, [50], 0, BF),           # more heads than a tile has rows: CUDA cores
+    (96, 1, 64, 16, 9, [300, 1000], 0, HF),     # one node a group, groups side by side
+    (8, 8, 128, 512, 4, [1500, 511, 512], 0, BF),
+    (1, 1, 128, 128, 2, [70001], 0, BF),
+    (2, 1, 64, 16, 6, [40003, 3], 4096, HF),
+    (4, 1, 64, 16, 700, [10], 0, BF),           # 2800 rows of a KV head: several sets of groups
+]
+
+
+@pytest.mark.parametrize("Hq,H,D,S,T,ctx,width,dtype", SHAPES)
+def test_schedule_shapes(Hq, H, D, S, T, ctx, width, dtype):
+    g = torch.Generator().manual_seed(T + Hq)
+    n = len(ctx)
+    nodes = [max(1, T - i % 2) for i in range(n)]
+    kp, vp, table, seq, ks, vs = build([c + m for c, m in zip(ctx, nodes)], H, S, D, dtype, seed=Hq + S)
+    if width:
+        table = torch.nn.functional.pad(table, (0, width - table.shape[1]), value=-1)
+    q = torch.randn(n, Hq, T, D, generator=g).to(dtype)
+    out, lse = tree_attention(q.cuda(), kp, vp, table, seq, num_nodes=torch.tensor(nodes).cuda(), return_lse=True)
+    if T * Hq * sum(ctx) < 3e6:
+        check(out, lse, q, ks, vs, nodes, 1 / math.sqrt(D), dtype)
+        return
+    pick = sorted({0, 1, T // 2, T - 1} & set(range(min(nodes))))  # some rows of large cases
+    for t in pick:
+        for i in range(n):
+            m = nodes[i]
+            kk, vv = ks[i][:, :len(ks[i][0]) - m + t + 1], vs[i][:, :len(vs[i][0]) - m + t + 1]
+            check(out[i:i + 1, :, t:t + 1], lse[i:i + 1, :, t:t + 1], q[i:i + 1, :, t:t + 1], [kk], [vv], [1],
+                  1 / math.sqrt(D), dtype)
+
+
+@pytest.mark.parametrize("dtype,D,S", [(BF, 128, 64), (HF, 64, 16), (FP, 64, 16)])
+@pytest.mark.parametrize("up", [True, False])
+def test_scores_that_grow_or_fall_along_the_cache(dtype, D, S, up):
+    """The reference of the weights changes again and again, or never after the first tile."""
+    T, n = 5, 1700
+    kp, vp, table, seq, ks, vs = build([n], 1, S, D, dtype, fill=0.0)
+    ramp = torch.linspace(-1, 1, n) if up else torch.linspace(1, -1, n)
+    k = (0.1 * torch.from_numpy(ks[0][0]) + 6.0 * ramp[:, None]).to(dtype)
+    for x in range(n):
+        kp[int(table[0, x // S]), 0, x % S] = k[x].cuda()
+    q = (torch.rand(1, 2, T, D) + 0.5).to(dtype)
+    out, lse = tree_attention(q.cuda(), kp, vp, table, seq, return_lse=True)
+    check(out, lse, q, [k.float().numpy()[None]], vs, [T], 1 / math.sqrt(D), dtype)
+
+
+@pytest.mark.parametrize("dtype,S,D", [(BF, 16, 128), (HF, 64, 64)])
+def test_infinite_scores(dtype, S, D):
+    """+inf among the seen scores gives NaN as softmax does; -inf is a weight of 0."""
+    kp, vp, table, seq, ks, vs = build([300], 1, S, D, dtype)
+    q = torch.ones(1, 1, 2, D, dtype=dtype, device="cuda")
+    clean = tree_attention(q, kp, vp, table, seq)
+    page, slot = int(table[0, 37 // S]), 37 % S
+    keep = kp[page, 0, slot].clone()
+    kp[page, 0, slot] = math.inf
+    assert torch.isnan(tree_attention(q, kp, vp, table, seq)).all()
+    kp[page, 0, slot] = -math.inf
+    low = tree_attention(q, kp, vp, table, seq)
+    there = np.ones(300, dtype=bool)
+    there[37] = False
+    w, wl, absv, absqk = oracle_attention(q[0].float().cpu().numpy(), ks[0], vs[0], 2, D ** -0.5, there=there)
+    lo, _ = bounds(300, D, dtype, absqk, absv, w, wl)
+    assert (np.abs(low[0].float().cpu().numpy() - w) <= lo).all()
+    kp[page, 0, slot] = keep
+    assert torch.equal(tree_attention(q, kp, vp, table, seq), clean)
+
+
 @pytest.mark.parametrize("dtype,S,D", [(BF, 16, 128), (HF, 64, 64), (FP, 16, 64), (BF, 24, 128)])
 def test_strides_rows_and_out(dtype, S, D):
     """Slot-major pages, a query in [n, T, H, D] memory, an output view, rows out of order and twice,

@@ -156,3 +156,15 @@ def test_oracle_attention_is_softmax():
     s = (torch.from_numpy(q) @ kt.transpose(1, 2) * 0.3).masked_fill(~seen, -torch.inf)
     assert np.allclose(out, (torch.softmax(s, -1) @ vt).numpy(), atol=1e-12)
     assert np.allclose(lse, torch.logsumexp(s, -1).numpy(), atol=1e-12)
+
+
+def test_operators_are_registered_with_fakes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    for name in ("tree_attn", "pages_extend", "pages_write", "pages_compact", "pages_fork", "pages_truncate"):
+        assert hasattr(torch.ops.cab, name), name
+    with FakeTensorMode():
+        q = torch.empty(3, 8, 5, 128, dtype=torch.bfloat16, device="cuda")
+        k = torch.empty(20, 2, 16, 128, dtype=torch.bfloat16, device="cuda")
+        i = torch.empty(3, 7, dtype=torch.int32, device="cuda")
+        out, lse = torch.ops.cab.tree_attn(q, k, k, i, i[:, 0], None, None, None, None, 0.0)
+        assert out.shape == q.shape and out.dtype == q.dtype and lse.shape == (3, 8, 5) and lse.dtype == torch.float32
