@@ -82,17 +82,22 @@ class PagedKVCache:
             _lib.check(L.cab_pages_update_workspace_size(self._c, n, nbytes), "cab_pages_update_workspace_size")
             size = self._sizes[n] = nbytes.value
         ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+        keep_ptr = num_ptr = None
         keep_bytes = keep_stride = keep_cols = num_stride = 0
         if keep is not None:
-            keep_bytes, keep_stride, keep_cols = keep.element_size(), keep.stride(0), keep.shape[1]
-            num_stride = 0 if keep_num is None else keep_num.stride(0)
-        call_on(self.device, "cab_pages_update", L.cab_pages_update, self._c, _lib.ptr(src), _lib.ptr(dst), n,
-                _lib.ptr(start), start_value, _lib.ptr(keep), keep_bytes, keep_stride, keep_cols, _lib.ptr(keep_num),
-                num_stride, _lib.ptr(grow), grow_value, int(copies), ws.data_ptr(), size)
+            keep_ptr, keep_bytes, keep_stride, keep_cols = keep.data_ptr(), keep.element_size(), keep.stride(0), keep.shape[1]
+            if keep_num is not None:
+                num_ptr, num_stride = keep_num.data_ptr(), keep_num.stride(0)
+        call_on(self.device, "cab_pages_update", L.cab_pages_update, self._c, None if src is None else src.data_ptr(),
+                None if dst is None else dst.data_ptr(), n, None if start is None else start.data_ptr(), start_value,
+                keep_ptr, keep_bytes, keep_stride, keep_cols, num_ptr, num_stride,
+                None if grow is None else grow.data_ptr(), grow_value, copies, ws.data_ptr(), size)
 
     def _rows(self, rows, name: str = "rows"):
+        if rows is None:
+            return None, self.num_rows
         rows = int32_vector(rows, None, name, self.device)
-        return rows, (self.num_rows if rows is None else rows.shape[0])
+        return rows, rows.shape[0]
 
     def extend(self, num_new: Union[int, torch.Tensor], rows: Optional[torch.Tensor] = None) -> None:
         """Room for ``num_new`` more tokens of each row, to be written by ``write``."""
@@ -160,7 +165,7 @@ class PagedKVCache:
               rows: Optional[torch.Tensor] = None) -> None:
         """Keys and values ``[n, Hkv, T, D]`` of each row's newest ``num_new`` (default T) tokens; tokens
         t >= num_new[i] are not written. Rows must differ."""
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != self.dtype or v.dtype != self.dtype:
+        if k.dim() != 4 or k.shape != v.shape or k.dtype is not self.dtype or v.dtype is not self.dtype:
             raise ValueError(f"k and v must be [n, Hkv, T, D] of the cache's dtype {self.dtype}")
         if k.device != self.device or v.device != self.device:
             raise ValueError(f"k and v must be on {self.device}")
@@ -175,12 +180,16 @@ class PagedKVCache:
         num_new = int32_vector(num_new, n, "num_new", self.device)
         if n == 0 or T == 0:
             return
-        if k.stride(3) != 1:
+        ks, vs = k.stride(), v.stride()
+        if ks[3] != 1:
             k = k.contiguous()
-        if v.stride(3) != 1:
+            ks = k.stride()
+        if vs[3] != 1:
             v = v.contiguous()
+            vs = v.stride()
         call_on(self.device, "cab_pages_write", _lib.lib().cab_pages_write, self._c, layer, k.data_ptr(), v.data_ptr(),
-                n, T, _lib.strides(*k.stride()[:3]), _lib.strides(*v.stride()[:3]), _lib.ptr(rows), _lib.ptr(num_new), T)
+                n, T, _lib.strides(ks[0], ks[1], ks[2]), _lib.strides(vs[0], vs[1], vs[2]),
+                None if rows is None else rows.data_ptr(), None if num_new is None else num_new.data_ptr(), T)
 
     def attend(self, layer: int, q: torch.Tensor, parents: Optional[torch.Tensor] = None,
                tree_mask: Optional[torch.Tensor] = None, num_nodes: Optional[torch.Tensor] = None,

@@ -20,7 +20,8 @@ import torch
 
 from .. import _lib
 
-_current_device = torch.cuda.current_device
+_current_device = torch._C._cuda_getDevice  # the device is initialised: the tensors are on it
+_INTS, _BOOLS = (torch.int32, torch.int64), (torch.bool, torch.uint8)
 
 
 def describe_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -63,11 +64,12 @@ def int32_vector(t: Optional[torch.Tensor], n: Optional[int], name: str, device)
     """``t`` as a contiguous int32 vector of ``n`` entries on ``device`` (int64 is converted)."""
     if t is None:
         return None
-    if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or (n is not None and t.shape[0] != n):
+    shape, dtype = t.shape, t.dtype
+    if len(shape) != 1 or (n is not None and shape[0] != n) or (dtype is not torch.int32 and dtype is not torch.int64):
         raise ValueError(f"{name} must be an int32 or int64 tensor [{'n' if n is None else n}]")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}")
-    if t.dtype == torch.int32 and t.is_contiguous():
+    if dtype is torch.int32 and t.is_contiguous():
         return t
     return t.to(torch.int32).contiguous()
 
@@ -86,51 +88,60 @@ def call_on(device: torch.device, name: str, fn, *args) -> None:
 
 def attend_cache(cache, device, dtype, layer: int, q: torch.Tensor, parents=None, tree_mask=None, num_nodes=None,
                  rows=None, softmax_scale=None, out=None, return_lse: bool = False):
-    """``tree_attention`` on a described cache (``describe_cache``)."""
-    if q.dim() != 4 or q.dtype != dtype:
+    """``tree_attention`` on a described cache (``describe_cache``). Written for few host
+    microseconds: a decode step of a short cache takes less time on the device than here."""
+    shape = q.shape
+    if len(shape) != 4 or q.dtype is not dtype:
         raise ValueError(f"q must be [n, Hq, T, D] of the cache's dtype {dtype}")
     if q.device != device:
         raise ValueError(f"q must be on {device}")
-    n, Hq, T, D = q.shape
+    n, Hq, T, D = shape
     if D != cache.dim or Hq == 0 or Hq % cache.heads:
         raise ValueError(f"q must have D = {cache.dim} and a multiple of {cache.heads} heads")
     if not 0 <= layer < cache.layers:
         raise ValueError(f"layer {layer} of {cache.layers}")
-    rows = int32_vector(rows, n, "rows", device)
-    if rows is None and n > cache.rows:
+    rows_ptr = nodes_ptr = parents_ptr = mask_ptr = None
+    if rows is not None:
+        rows = int32_vector(rows, n, "rows", device)
+        rows_ptr = rows.data_ptr()
+    elif n > cache.rows:
         raise ValueError(f"{n} sequences, {cache.rows} rows")
-    num_nodes = int32_vector(num_nodes, n, "num_nodes", device)
+    if num_nodes is not None:
+        num_nodes = int32_vector(num_nodes, n, "num_nodes", device)
+        nodes_ptr = num_nodes.data_ptr()
     parents_stride = mask_stride = 0
     if parents is not None:
         if tree_mask is not None:
             raise ValueError("give parents or tree_mask, not both")
-        if parents.dtype not in (torch.int32, torch.int64) or tuple(parents.shape) not in ((T,), (n, T)):
+        if parents.dtype not in _INTS or parents.shape not in ((T,), (n, T)):
             raise ValueError(f"parents must be int32 or int64 [{T}] or [{n}, {T}]")
         if parents.device != device:
             raise ValueError(f"parents must be on {device}")
-        parents = parents.to(torch.int32).contiguous()
-        parents_stride = T if parents.dim() == 2 else 0
-    if tree_mask is not None:
-        if tree_mask.dtype not in (torch.bool, torch.uint8) or tuple(tree_mask.shape) not in ((T, T), (n, T, T)):
+        if parents.dtype is not torch.int32 or not parents.is_contiguous():
+            parents = parents.to(torch.int32).contiguous()
+        parents_ptr, parents_stride = parents.data_ptr(), (T if parents.dim() == 2 else 0)
+    elif tree_mask is not None:
+        if tree_mask.dtype not in _BOOLS or tree_mask.shape not in ((T, T), (n, T, T)):
             raise ValueError(f"tree_mask must be bool [{T}, {T}] or [{n}, {T}, {T}]")
         if tree_mask.device != device:
             raise ValueError(f"tree_mask must be on {device}")
-        tree_mask = tree_mask.contiguous()
-        mask_stride = T * T if tree_mask.dim() == 3 else 0
-    scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
+        if not tree_mask.is_contiguous():
+            tree_mask = tree_mask.contiguous()
+        mask_ptr, mask_stride = tree_mask.data_ptr(), (T * T if tree_mask.dim() == 3 else 0)
+    scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
+    if not 0.0 < scale < math.inf:
         raise ValueError("softmax_scale must be positive and finite")
     if out is None:
-        out = torch.empty(n, Hq, T, D, dtype=dtype, device=device)
-    elif tuple(out.shape) != (n, Hq, T, D) or out.dtype != dtype or out.device != device or out.stride(3) != 1:
+        out = torch.empty(n, Hq, T, D, dtype=dtype, device=device)  # sizes one by one parse faster than a tuple
+    elif out.shape != shape or out.dtype is not dtype or out.device != device or out.stride(3) != 1:
         raise ValueError("out must be [n, Hq, T, D] of q's dtype and device with a dense last dimension")
     lse = torch.empty(n, Hq, T, dtype=torch.float32, device=device) if return_lse else None
     if n == 0 or T == 0:
         return (out, lse) if return_lse else out
-    qs, es = q.stride(), q.element_size()
-    if qs[3] != 1 or any(x <= 0 or (x * es) % 16 for x in qs[:3]) or q.data_ptr() % 16:
+    s0, s1, s2, s3 = q.stride()
+    if s3 != 1 or (s0 | s1 | s2) & (16 // q.element_size() - 1) or not (s0 > 0 and s1 > 0 and s2 > 0) or q.data_ptr() & 15:
         q = q.clone(memory_format=torch.contiguous_format)  # contiguous() would return a misaligned dense view
-        qs = q.stride()
+        s0, s1, s2, _ = q.stride()
     L = _lib.lib()
     nbytes = cache.sizes.get((n, Hq, T))
     if nbytes is None:
@@ -139,10 +150,11 @@ def attend_cache(cache, device, dtype, layer: int, q: torch.Tensor, parents=None
             _lib.check(L.cab_tree_attn_workspace_size(cache, n, Hq, T, size), "cab_tree_attn_workspace_size")
         nbytes = cache.sizes[(n, Hq, T)] = size.value
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    os = out.stride()
+    o0, o1, o2, _ = out.stride()
     call_on(device, "cab_tree_attn_fwd", L.cab_tree_attn_fwd, cache, layer, q.data_ptr(), out.data_ptr(),
-            None if lse is None else lse.data_ptr(), n, Hq, T, _lib.strides(*qs[:3]), _lib.strides(*os[:3]), _lib.ptr(rows), _lib.ptr(num_nodes), _lib.ptr(parents), parents_stride,
-            _lib.ptr(tree_mask), mask_stride, scale, None if ws is None else ws.data_ptr(), nbytes)
+            lse.data_ptr() if return_lse else None, n, Hq, T, _lib.strides(s0, s1, s2), _lib.strides(o0, o1, o2),
+            rows_ptr, nodes_ptr, parents_ptr, parents_stride, mask_ptr, mask_stride, scale,
+            None if ws is None else ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 
 

@@ -227,10 +227,9 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
   // the keep lists: range, and the first entry that moves
   if (K > 0) {
     bool bad = false;
-    const int64_t total = K * n;
-    for (int64_t e = static_cast<int64_t>(me) * nt + tid; e < total; e += static_cast<int64_t>(nc) * nt) {
-      const int i = static_cast<int>(e / K);
-      const int x = static_cast<int>(e - i * K);
+    const uint32_t cols = static_cast<uint32_t>(K), listed = cols * n;  // below 2^31
+    for (uint32_t e = me * nt + tid; e < listed; e += nc * nt) {
+      const int i = static_cast<int>(e / cols), x = static_cast<int>(e - i * cols);
       if (x < s_content[i] - s_start[i]) {
         const int64_t v = keep_at(p.keep, p.keep64, i * p.keep_stride + x);
         bad |= v < 0 || v >= s_room[i];
@@ -648,6 +647,7 @@ extern "C" int cab_pages_update(const cab_page_cache* cache, const int32_t* src,
   if (int rc = check_pairs(cache, n)) return rc;
   if (!src && n > cache->rows) return fail(CAB_ERR_INVALID_ARG, "pages_update: %lld pairs without source rows, %lld rows", (long long)n, (long long)cache->rows);
   if (keep_cols < 0 || keep_cols >= (int64_t)1 << 31) return fail(CAB_ERR_INVALID_ARG, "pages_update: bad number of keep columns");
+  if (n * keep_cols >= (int64_t)1 << 31) return fail(CAB_ERR_UNSUPPORTED, "pages_update: more than 2^31 list entries a call");
   if (keep_cols > 0 && (!keep || (keep_bytes != 4 && keep_bytes != 8))) return fail(CAB_ERR_INVALID_ARG, "pages_update: keep must be int32 or int64");
   if (keep_cols > 0 && !copies) return fail(CAB_ERR_INVALID_ARG, "pages_update: a keep list needs copies");
   if (grow_value < 0) return fail(CAB_ERR_INVALID_ARG, "pages_update: negative growth");

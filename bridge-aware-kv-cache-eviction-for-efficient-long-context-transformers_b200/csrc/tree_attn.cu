@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(kSimtThreads) simt_kernel(const __grid_constan
   float* sP = sV + kKeysTile * Dp;   // [rows][32]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int R = p.G * p.T, tiles_r = (R + kRowsTile - 1) / kRowsTile;
   const int unit = blockIdx.x, split = blockIdx.y;
   const int rt = unit % tiles_r, hk = (unit / tiles_r) % p.Hkv, i = unit / (tiles_r * p.Hkv);
@@ -1325,7 +1326,7 @@ int launch_simt(const Params& p, int64_t units, cudaStream_t st) {
   const int Dp = (p.D + 3) & ~3;
   const size_t smem = static_cast<size_t>(4 * RW * (Dp + 32) + kKeysTile * (Dp + 4) + kKeysTile * Dp) * 4;
   if (smem > 48 * 1024) cudaFuncSetAttribute(simt_kernel<T, DC, RW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  simt_kernel<T, DC, RW><<<dim3(static_cast<unsigned>(units), static_cast<unsigned>(p.splits)), kSimtThreads, smem, st>>>(p);
+  pages::launch_after(simt_kernel<T, DC, RW>, dim3(static_cast<unsigned>(units), static_cast<unsigned>(p.splits)), kSimtThreads, st, smem, 1, p);
   if (int rc = check_launch("tree_attn simt_kernel")) return rc;
   if (p.splits == 1) return CAB_OK;
   pages::launch_after(simt_join_kernel<T, DC>, dim3(static_cast<unsigned>(units * RW)), kSimtThreads, st, 0, 1, p, 4 * RW);
