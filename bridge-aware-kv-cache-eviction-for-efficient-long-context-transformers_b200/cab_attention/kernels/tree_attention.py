@@ -71,7 +71,12 @@ def int32_vector(t: Optional[torch.Tensor], n: Optional[int], name: str, device)
         raise ValueError(f"{name} must be on {device}")
     if dtype is torch.int32 and t.is_contiguous():
         return t
-    return t.to(torch.int32).contiguous()
+    return to_int32(t)
+
+
+def to_int32(t: torch.Tensor) -> torch.Tensor:
+    """As contiguous int32; what does not fit stays out of range instead of wrapping around."""
+    return (t if t.dtype is torch.int32 else t.clamp(-1, 2 ** 31 - 1).to(torch.int32)).contiguous()
 
 
 def call_on(device: torch.device, name: str, fn, *args) -> None:
@@ -118,7 +123,7 @@ def attend_cache(cache, device, dtype, layer: int, q: torch.Tensor, parents=None
         if parents.device != device:
             raise ValueError(f"parents must be on {device}")
         if parents.dtype is not torch.int32 or not parents.is_contiguous():
-            parents = parents.to(torch.int32).contiguous()
+            parents = to_int32(parents)
         parents_ptr, parents_stride = parents.data_ptr(), (T if parents.dim() == 2 else 0)
     elif tree_mask is not None:
         if tree_mask.dtype not in _BOOLS or tree_mask.shape not in ((T, T), (n, T, T)):
@@ -169,7 +174,7 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
 
     ``parents`` int ``[n, T]`` or ``[T]`` (each node's parent, before it; negative: none), or
     ``tree_mask`` bool ``[n, T, T]`` or ``[T, T]`` (which node sees which), or neither: node t
-    sees nodes 0..t, so ``T = 1`` is a decode step. ``num_nodes [n]`` (default T): nodes of each
+    sees nodes 0..t, so ``T = 1`` is a decode step (``parents``: at most 1024 nodes). ``num_nodes [n]`` (default T): nodes of each
     sequence. Returns ``out [n, Hq, T, D]``, with ``return_lse`` also the natural-log sum-exp
     ``[n, Hq, T]`` fp32.
 

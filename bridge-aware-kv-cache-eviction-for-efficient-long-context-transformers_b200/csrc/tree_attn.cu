@@ -27,6 +27,7 @@ namespace tree {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMaxTree = 1024;  // nodes of a tree given by parents: a query walks up its ancestors
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -1195,9 +1196,10 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ Param
   }
   __syncthreads();
   const int c0 = s_c0, c1 = s_c1;
+  // Every block waits, also one without work: a kernel launched behind this one takes its end for the end of both.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (c0 == c1) return;
   const int rr = blockIdx.y * (blockDim.x >> 5) + warp, t = grp * sh.nodes + rr / p.G;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (rr >= sh.nodes * p.G || t >= p.T) return;
   auto part = [&](int c) -> int64_t {  // the row's place in range c's partial slot
     return (2 * (static_cast<int64_t>(c) * sh.wide + side) + (c == c0 && !s_first ? 1 : 0)) * p.part_rows + rr;
@@ -1379,6 +1381,7 @@ extern "C" int cab_tree_attn_fwd(const cab_page_cache* cache, int64_t layer, con
   if (layer < 0 || layer >= cache->layers) return fail(CAB_ERR_INVALID_ARG, "tree_attn: layer %lld of %lld", (long long)layer, (long long)cache->layers);
   if (!rows && n > cache->rows) return fail(CAB_ERR_INVALID_ARG, "tree_attn: more sequences than rows");
   if (parents && tree_mask) return fail(CAB_ERR_INVALID_ARG, "tree_attn: parents or a mask, not both");
+  if (parents && T > kMaxTree) return fail(CAB_ERR_UNSUPPORTED, "tree_attn: %lld nodes given by parents (at most %d)", (long long)T, kMaxTree);
   if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale)) return fail(CAB_ERR_INVALID_ARG, "tree_attn: softmax_scale must be > 0 and finite");
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] < 0 || o_strides[i] < 0) return fail(CAB_ERR_INVALID_ARG, "tree_attn: negative stride");

@@ -392,7 +392,7 @@ CAB_API int cab_tree_attn_workspace_size(const cab_page_cache* cache, int64_t n,
  * {n, h, t}. Sequence i is row rows[i] (NULL: i); its last m = num_nodes[i] (NULL: T) cached
  * tokens are its nodes, whose queries are q[i, :, :m]. A node sees every earlier token of the
  * cache and, among the nodes, its ancestors and itself (parents [n,T] with row stride
- * parents_stride, 0 = one tree for all; parents[t] < t, negative: a root), or those with
+ * parents_stride, 0 = one tree for all; parents[t] < t, else a root; T <= 1024), or those with
  * tree_mask[i,t,u] != 0 (uint8 [n,T,T], stride mask_stride, 0 = one mask), or u <= t when
  * both are NULL. softmax over the seen tokens; a query that sees none and the queries past m
  * give 0 (lse -inf). lse [n,Hq,T] fp32 natural log, may be NULL. A sequence whose row is out

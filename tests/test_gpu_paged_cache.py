@@ -134,6 +134,8 @@ def test_refusals_leave_the_cache_as_it_was():
         (lambda: c.extend(97, dev([2])), 2),                             # 6 pages a row
         (lambda: c.extend(1, dev([4])), 4),
         (lambda: c.extend(1, dev([-1])), 4),
+        (lambda: c.extend(1, dev([2 ** 32], torch.int64)), 4),           # not row 0
+        (lambda: c.truncate(dev([2 ** 32 + 3], torch.int64), dev([0])), 8),
         (lambda: c.extend(1, dev([1, 1])), 4),
         (lambda: c.fork(dev([0, 0]), dev([2, 2])), 4),
         (lambda: c.truncate(41, dev([0])), 8),
@@ -262,3 +264,40 @@ def test_graph_replay_and_side_stream():
         o.update(pairs([0, 1, 2, 3], start=at, keep=[[0, 2], [1], [0, 1], [0, 2]]))
     same(c, o)
     c.check()
+
+
+@pytest.mark.parametrize("S,D,lens", [(16, 64, [3, 40, 0, 17]), (16, 128, [900, 5, 700, 60])])
+def test_queued_steps_equal_waited_ones(S, D, lens):
+    """Decode steps queued without a wait, so that each kernel is launched while those before it run,
+    give what the same steps give with a wait after every call."""
+    def steps(wait):
+        c, _ = make(L=1, P=400, S=S, D=D, R=4, W=64, seed=1)
+        pause = torch.cuda.synchronize if wait else (lambda: None)
+        g = torch.Generator(device="cuda").manual_seed(4)
+        kv = torch.randn(8, 4, 2, 3, D, device="cuda", generator=g).to(torch.bfloat16)
+        first = torch.randn(4, 2, max(lens), D, device="cuda", generator=g).to(torch.bfloat16)
+        c.extend(dev(lens))
+        pause()
+        c.write(0, first, first, dev(lens))
+        pause()
+        outs = []
+        for i in range(40):
+            n = c.seq_lens.clone()
+            c.extend(3)
+            pause()
+            c.write(0, kv[i % 8], kv[(i + 3) % 8])
+            pause()
+            outs.append(c.attend(0, kv[(i + 1) % 8].repeat_interleave(2, 1)))
+            pause()
+            c.compact(dev([[0, 2], [1, 0], [0, 0], [2, 1]]), dev([2, 1, 2, 1]), start=n)
+            pause()
+            if i % 5 == 4:
+                c.fork(dev([0, 1]), dev([2, 3]))
+                pause()
+        c.check()
+        return outs + [c.k_pages, c.v_pages, c.block_table, c.seq_lens, c.ref_counts]
+
+    want = steps(True)
+    for _ in range(3):
+        for x, y in zip(steps(False), want):
+            assert torch.equal(x, y)

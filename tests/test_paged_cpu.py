@@ -76,6 +76,7 @@ def test_c_abi_refusals(lib):
     assert attend(fake_cache(), n=5) == 1
     assert attend(fake_cache(), layer=1) == 1
     assert attend(fake_cache(), parents=fake, mask=fake) == 1
+    assert attend(fake_cache(), T=1025, parents=fake) == 2
     for scale in (0.0, -1.0, float("inf"), float("nan")):
         assert attend(fake_cache(), scale=scale) == 1
     assert attend(fake_cache(dim=257)) == 2
