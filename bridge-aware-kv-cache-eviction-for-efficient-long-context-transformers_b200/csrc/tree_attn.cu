@@ -422,7 +422,7 @@ constexpr int kBufs = 3;
 constexpr uint32_t kTmemO = 384;
 constexpr int kMaxShare = 4;
 constexpr int kLostRing = 16;  // tiles between the K loads and the softmax, at most kStages + 3
-constexpr int kUnitCost = 3;
+constexpr int kUnitCost = 4;
 constexpr int kWholeTiles = 4;  // rows of at most this many tiles are not cut: no join
 
 template <int D>
@@ -510,7 +510,8 @@ __device__ __forceinline__ int64_t range_start(int64_t total, int64_t ranges, in
   return x >> 32 == 0 ? static_cast<uint32_t>(x) / static_cast<uint32_t>(ranges) : x / static_cast<uint64_t>(ranges);
 }
 __device__ __forceinline__ int range_count(int64_t total, int most, int least) {
-  return static_cast<int>(min(static_cast<int64_t>(most), (total + least - 1) / least));
+  if (total >= static_cast<int64_t>(most) * least) return most;
+  return (static_cast<int>(total) + least - 1) / least;
 }
 
 // Warp-wide: the weight of all units and, if `count` is not 0, of this range: the sequence in which its
@@ -768,19 +769,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int range = blockIdx.x / sh.wide, side = blockIdx.x % sh.wide;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < 4 * kStages; ++s) mbar_init(&k_full[s], 1);
-    for (int s = 0; s < kBufs; ++s) {
-      mbar_init(&s_full[s], 2);  // the product, and the issuer itself: it passes on what the K loader wrote
-      mbar_init(&p_full[s], 4);
-      mbar_init(&buf_free[s], 1);
+  if (warp == 0) {
+    // The barriers lie in one row: K / V stages, s_full (2: the product, and the issuer itself, which passes
+    // on what the K loader wrote), p_full (4 warps), buf_free, q_full, q_free, drain; a lane each.
+    constexpr int kAll = 4 * kStages + 3 * kBufs + 4;
+    for (int i = lane; i < kAll; i += 32) {
+      const int j = i - 4 * kStages;
+      mbar_init(&k_full[i], j < 0 ? 1 : j < kBufs ? 2 : j < 2 * kBufs ? 4 : 1);
     }
-    mbar_init(q_full, 1);
-    mbar_init(q_free, 1);
-    mbar_init(&drain[0], 1);
-    mbar_init(&drain[1], 1);
-    *abort_flag = 0;
-    *odd_seg = 0;
+    if (lane == 0) {
+      *abort_flag = 0;
+      *odd_seg = 0;
+    }
     fence_barrier_init();
   }
   if (threadIdx.x == 32) {
