@@ -134,7 +134,10 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int n, int64_t* tmp, in
 // One cluster (1 or 8 CTAs) makes the whole update. The work is a few passes over small integer
 // arrays (use counts, keep lists, table rows), bound by the latency of dependent loads, so the
 // passes are separated by cluster barriers instead of launches, what the CTAs tell one another goes through
-// distributed shared memory, and each pass has its loads in flight together.
+// distributed shared memory, and each pass has its loads in flight together. About 12,000 clocks with few
+// rows, 20,000 with 32 rows of 500 pages; the code runs once a launch, so its size costs as much as its
+// loads (unrolling the entry rounds four times instead of two: 20.5 instead of 17.8 us for a fork of 32
+// beams with its copies), and one CTA of 1024 threads for everything took twice as long on 32 rows.
 constexpr int kWordRounds = 2;  // ballot words of free pages a lane of a warp holds at a time
 
 __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_constant__ UpdateParams p) {
@@ -415,7 +418,8 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
 // Moves up to 32 tokens' K and V of one (layer, head) per warp: lane t finds where token t
 // comes from and goes to (three dependent small loads for 32 tokens at once), then the warp
 // moves the tokens' rows in vectors, kBatch loads of K and of V in flight per lane. Bound by
-// HBM: each moved value is read and written once.
+// HBM: each moved value is read and written once. 2 x 6400 tokens of 8 heads of 128 kept out of 128,000:
+// 105 MB in 18 us, 5.8 TB/s; writing 2 x 32,768 tokens: 537 MB in 85 us, 6.3 TB/s (copy rate 6.55).
 struct RowSpan {
   int64_t ksrc, vsrc, kdst, vdst;  // element offsets of a token's row
 };

@@ -112,7 +112,9 @@ __device__ __forceinline__ int key_limit(const Params& p, const Seq& s, int t_la
 // warp reductions; for the output a lane owns the columns lane + 32 c. Four threads fetch a key: its page is
 // looked up once, then its K and V rows come in 4-element vectors. Bound by shared-memory reads: per 4 dims
 // 4 wavefronts of keys and one of each row's query for 4 * RW multiply-adds, so many rows take RW = 8, few
-// (up to 16) RW = 4 to spread them over the warps.
+// (up to 16) RW = 4 to spread them over the warps. Few rows are bound by latency: 3 rows of 0.9 to 1.5k
+// tokens, 8 heads of 64, 5 nodes, float32: 23 us with the join (45 us with scalar fetches and one warp-wide
+// sum per tile).
 constexpr int kKeysTile = 32, kSimtThreads = 128;
 
 template <typename T>
@@ -412,6 +414,13 @@ __global__ void __launch_bounds__(kSimtThreads) simt_join_kernel(const __grid_co
 // length are masked per row by a 64-bit word, and V rows past the length and values of nodes that
 // are not finite are zeroed in shared memory, so that 0 * NaN cannot enter a product; a seen value
 // that is not finite is added back to the rows that see it (fix_up).
+//
+// Measured (B200): 32 rows of 0.8 to 8k tokens, 32 / 8 heads of 128, one token, 16-token pages: 606 MB
+// from HBM (each key and value once) in 111 us, 5.5 TB/s = 0.83 of the copy rate; the rest is the first tiles'
+// latency (table, page and tile one after the other, 7 us), and the join. 4 trees of 64 nodes over 65,536
+// tokens (275 GFLOP, 256 rows a KV head): 265 us = 1.04 PFLOP/s alone, 0.33 ms in a loop, where the 1 kW cap
+// lowers the clock to 1.3 - 1.6 GHz; 1.08 GB from HBM, so the CTAs side by side share each tile through L2.
+// Before that: one tile a time on two streams with an O each 407 us; 64 keys a thread 361 us.
 //
 // Every mbarrier has one waiter per phase and direction, or its next phase needs the waiter's own
 // next step, so parity waits never meet a barrier two phases on.
