@@ -107,7 +107,8 @@ __device__ __forceinline__ int key_limit(const Params& p, const Seq& s, int t_la
 
 // ------------------------------------------------------------------ CUDA-core path
 // fp32 arithmetic for any type, page size and head_dim <= 256: float32 caches, and shapes the
-// tensor-core path does not take. One CTA per (sequence, KV head, 4 * RW rows, key split). A warp
+// tensor-core path does not take. One CTA per (sequence, KV head, 4 * RW rows, key split).
+// (More than 8 rows, or rows that are not 8 columns on 16 bytes.) A warp
 // owns RW rows and a lane one key of the 32-key tile for the scores, so a row's maximum and sum are
 // warp reductions; for the output a lane owns the columns lane + 32 c. Four threads fetch a key: its page is
 // looked up once, then its K and V rows come in 4-element vectors. Bound by shared-memory reads: per 4 dims
@@ -335,6 +336,169 @@ __global__ void __launch_bounds__(kSimtThreads) simt_kernel(const __grid_constan
       for (int c = 0; c < DC; ++c)
         if (lane + 32 * c < p.D) p.part_o[slot * p.D + lane + 32 * c] = acc[r][c];
       if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m[r], l[r]);
+    }
+  }
+}
+
+// Up to 8 rows: no tile in shared memory, the products are vector by vector. LK = D / 8 lanes (8, 16 or
+// 32) hold 8 columns of the queries and sums each and take a key together: its K and V rows come straight
+// from global memory, the score is a sum over the lanes, and each group of lanes keeps a maximum, sums and
+// output of its own, joined at the end. A warp takes 32 keys at a time, whose pages its lanes look up
+// together. Bound by the loads in flight: two keys' rows a lane.
+constexpr int kFewRows = 8;
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const float4 a = Vec4<T>::widen(make_uint2(v.x, v.y)), b = Vec4<T>::widen(make_uint2(v.z, v.w));
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+}
+
+template <typename T, int LK, int RM>
+__global__ void __launch_bounds__(kSimtThreads) few_rows_kernel(const __grid_constant__ Params p) {
+  constexpr int kGroups = 32 / LK, kCols = 8 * LK;
+  __shared__ float s_acc[4][RM][kCols], s_m[4][RM], s_l[4][RM];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane / LK, col = (lane % LK) * 8;
+  const int R = p.G * p.T, unit = blockIdx.x, split = blockIdx.y, hk = unit % p.Hkv, i = unit / p.Hkv;
+  const Seq s = load_seq(p, i);
+  const int keys = s.len;
+  const int chunks = (keys + 31) / 32, per = (chunks + p.splits - 1) / p.splits;
+  const int c_lo = min(chunks, split * per), c_hi = min(chunks, c_lo + per);
+  const uint32_t S = static_cast<uint32_t>(p.page_size);
+  const int32_t* table = p.table + s.row * p.table_stride;
+  const bool there = col < p.D;
+  const T* kbase = static_cast<const T*>(p.k) + hk * p.ks[1] + col;
+  const T* vbase = static_cast<const T*>(p.v) + hk * p.vs[1] + col;
+  float q[RM][8], acc[RM][8], m[RM], l[RM];
+  uint32_t live = 0u;
+#pragma unroll
+  for (int r = 0; r < RM; ++r) {
+    const int t = r / p.G;
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[r][e] = acc[r][e] = 0.f;
+    if (r < R && t < s.m) {
+      live |= 1u << r;
+      const T* src = static_cast<const T*>(p.q) + i * p.qs[0] + (hk * p.G + r - t * p.G) * p.qs[1] + t * p.qs[2] + col;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[r][e] = there ? to_f32(src[e]) * p.scale_log2 : 0.f;
+    }
+  }
+  for (int c = c_lo + warp; c < c_hi; c += 4) {
+    const int mine = c * 32 + lane;
+    int page = -1;
+    uint32_t slot = 0u;
+    if (mine < keys) {
+      const uint32_t j = static_cast<uint32_t>(mine) / S;
+      slot = static_cast<uint32_t>(mine) - j * S;
+      page = table[j];
+      if (page >= p.pages) page = -1;
+    }
+#pragma unroll 1
+    for (int sub = 0; sub < LK; sub += 2) {
+      float kk[2][8], vv[2][8];
+      uint32_t vis[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int x = (sub + u) * kGroups + grp, key = c * 32 + x;
+        const int64_t pg = __shfl_sync(0xffffffffu, page, x), sl = __shfl_sync(0xffffffffu, slot, x);
+        vis[u] = pg < 0 ? 0u : live;
+        if (pg >= 0 && key >= s.ctx) {
+#pragma unroll 1
+          for (int r = 0; r < R; ++r)
+            if (live >> r & 1u && !sees(p, i, r / p.G, key - s.ctx)) vis[u] &= ~(1u << r);
+        }
+        if (vis[u] != 0u && there) {
+          load8(kbase + pg * p.ks[0] + sl * p.ks[2], kk[u]);
+          load8(vbase + pg * p.vs[0] + sl * p.vs[2], vv[u]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) kk[u][e] = vv[u][e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float x[RM];
+#pragma unroll
+        for (int r = 0; r < RM; ++r) {
+          x[r] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[r] = fmaf(q[r][e], kk[u][e], x[r]);
+        }
+#pragma unroll
+        for (int o = LK / 2; o; o >>= 1)
+#pragma unroll
+          for (int r = 0; r < RM; ++r) x[r] += __shfl_xor_sync(0xffffffffu, x[r], o);
+#pragma unroll
+        for (int r = 0; r < RM; ++r) {
+          if (!(vis[u] >> r & 1u) || x[r] == -INFINITY) continue;  // unseen, or a weight of 0
+          if (x[r] > m[r]) {
+            const float alpha = ex2(m[r] - x[r]);  // from -inf: 0
+            l[r] *= alpha;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[r][e] *= alpha;
+            m[r] = x[r];
+          }
+          const float w = ex2(x[r] - m[r]);
+          l[r] += w;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[r][e] = fmaf(w, vv[u][e], acc[r][e]);
+        }
+      }
+    }
+  }
+  // the groups of a warp, then the warps
+#pragma unroll
+  for (int r = 0; r < RM; ++r) {
+#pragma unroll
+    for (int o = LK; o < 32; o <<= 1) {
+      const float mo = __shfl_xor_sync(0xffffffffu, m[r], o), lo = __shfl_xor_sync(0xffffffffu, l[r], o);
+      const float mn = fmaxf(m[r], mo), ref = mn == -INFINITY ? 0.f : mn, a = ex2(m[r] - ref), b = ex2(mo - ref);
+      l[r] = l[r] * a + lo * b;
+      m[r] = mn;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[r][e] = acc[r][e] * a + __shfl_xor_sync(0xffffffffu, acc[r][e], o) * b;
+    }
+    if (lane < LK) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s_acc[warp][r][col + e] = acc[r][e];
+      if (lane == 0) {
+        s_m[warp][r] = m[r];
+        s_l[warp][r] = l[r];
+      }
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < R * kCols; e += kSimtThreads) {
+    const int r = e / kCols, d = e - r * kCols;
+    const float mm = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+    const float ref = mm == -INFINITY ? 0.f : mm;
+    float o = 0.f, ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float a = ex2(s_m[w][r] - ref);
+      o = fmaf(a, s_acc[w][r][d], o);
+      ll = fmaf(a, s_l[w][r], ll);
+    }
+    if (p.splits == 1) {
+      const int t = r / p.G, h = hk * p.G + r - t * p.G;
+      if (d < p.D)
+        static_cast<T*>(p.out)[i * p.os[0] + h * p.os[1] + t * p.os[2] + d] = from_f32<T>(ll != 0.f ? o / ll : 0.f);
+      if (p.lse && d == 0) p.lse[(static_cast<int64_t>(i) * p.Hq + h) * p.T + t] = (mm + log2f(ll)) * kLn2;
+    } else {
+      const int64_t slot = (static_cast<int64_t>(unit) * RM + r) * p.splits + split;
+      if (d < p.D) p.part_o[slot * p.D + d] = o;
+      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(mm, ll);
     }
   }
 }
@@ -1239,16 +1403,28 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ Param
 }
 
 // ------------------------------------------------------------------ host side
-inline int simt_rows(int64_t R) { return R <= 16 ? 16 : 32; }
-// Key splits: about four CTAs per SM, none without a tile of the longest row the table allows.
-inline int simt_splits(int64_t units, int64_t tokens) {
-  const int64_t want = (static_cast<int64_t>(current_sm_count()) * 4 + units - 1) / units;
-  return static_cast<int>(std::max<int64_t>(1, std::min({want, (tokens + kKeysTile - 1) / kKeysTile, (int64_t)64})));
+// Whether K and V rows can be read 8 columns at a time.
+inline bool rows_in_8(const cab_page_cache* c) {
+  const int64_t es = static_cast<int64_t>(dtype_size(static_cast<int>(c->dtype)));
+  if (c->dim % 8 != 0 || !aligned16(c->k_pages) || !aligned16(c->v_pages)) return false;
+  for (int i = 0; i < 4; ++i)
+    if (c->k_strides[i] * es % 16 != 0 || c->v_strides[i] * es % 16 != 0) return false;
+  return true;
+}
+// Rows of a CTA on the CUDA-core path.
+inline int simt_rows(const cab_page_cache* c, int64_t R) { return R <= kFewRows && rows_in_8(c) ? kFewRows : R <= 16 ? 16 : 32; }
+// Key splits: as many CTAs as fit the GPU at once (registers: 3 an SM with 32 rows, else 4; one more split
+// would be a second wave, 287 us instead of 238 for 2 x 128 nodes of 16 / 4 heads over 2000 tokens), none
+// without a tile of the longest row the table allows.
+inline int simt_splits(int64_t units, int64_t tokens, int rows) {
+  const int64_t want = static_cast<int64_t>(current_sm_count()) * (rows == 32 ? 3 : 4) / units;
+  const int least = rows == kFewRows ? 128 : kKeysTile;  // few rows: 32 keys for each warp
+  return static_cast<int>(std::max<int64_t>(1, std::min({want, (tokens + least - 1) / least, (int64_t)64})));
 }
 
 struct Layout {
   bool tc, whole;
-  int splits, part_rows, ctas;
+  int splits, part_rows, ctas, rows;
   int64_t units;
   size_t part_o, part_ml, total;
 };
@@ -1281,9 +1457,10 @@ inline Layout layout(const cab_page_cache* c, int64_t n, int64_t Hq, int64_t T) 
     L.total = L.part_ml + slots * 8;
     return L;
   }
-  const int64_t rows = simt_rows(R);
+  L.rows = simt_rows(c, R);
+  const int64_t rows = L.rows;
   L.units = n * c->heads * ((R + rows - 1) / rows);
-  L.splits = simt_splits(L.units, c->width * c->page_size);
+  L.splits = simt_splits(L.units, c->width * c->page_size, L.rows);
   if (L.splits > 1) {
     const size_t slots = static_cast<size_t>(L.units) * L.splits * rows;
     L.part_ml = (slots * D * 4 + 15) & ~size_t(15);
@@ -1344,18 +1521,27 @@ int launch_simt(const Params& p, int64_t units, cudaStream_t st) {
   return check_launch("tree_attn simt_join_kernel");
 }
 
-template <typename T, int DC>
-int launch_simt_rows(const Params& p, int64_t units, cudaStream_t st) {
-  return simt_rows(static_cast<int64_t>(p.G) * p.T) == 16 ? launch_simt<T, DC, 4>(p, units, st) : launch_simt<T, DC, 8>(p, units, st);
+template <typename T, int DC, int LK>
+int launch_simt_rows(const Params& p, const Layout& L, cudaStream_t st) {
+  if (L.rows == 16) return launch_simt<T, DC, 4>(p, L.units, st);
+  if (L.rows == 32) return launch_simt<T, DC, 8>(p, L.units, st);
+  const dim3 grid(static_cast<unsigned>(L.units), static_cast<unsigned>(p.splits));
+  const int R = p.G * p.T;  // fewer rows, fewer registers and more loads in flight
+  if (R <= 2) pages::launch_after(few_rows_kernel<T, LK, 2>, grid, kSimtThreads, st, 0, 1, p);
+  else pages::launch_after(few_rows_kernel<T, LK, kFewRows>, grid, kSimtThreads, st, 0, 1, p);
+  if (int rc = check_launch("tree_attn few_rows_kernel")) return rc;
+  if (p.splits == 1) return CAB_OK;
+  const int rows = R <= 2 ? 2 : kFewRows;
+  pages::launch_after(simt_join_kernel<T, DC>, dim3(static_cast<unsigned>((L.units * rows + 3) / 4)), kSimtThreads, st, 0, 1, p, rows);
+  return check_launch("tree_attn simt_join_kernel");
 }
 
 template <typename T>
-int launch_simt_d(const Params& p, int64_t units, cudaStream_t st) {
-  if (p.D <= 64) return launch_simt_rows<T, 2>(p, units, st);
-  if (p.D <= 128) return launch_simt_rows<T, 4>(p, units, st);
-  return launch_simt_rows<T, 8>(p, units, st);
+int launch_simt_d(const Params& p, const Layout& L, cudaStream_t st) {
+  if (p.D <= 64) return launch_simt_rows<T, 2, 8>(p, L, st);
+  if (p.D <= 128) return launch_simt_rows<T, 4, 16>(p, L, st);
+  return launch_simt_rows<T, 8, 32>(p, L, st);
 }
-
 
 inline int check_sizes(const cab_page_cache* c, int64_t n, int64_t Hq, int64_t T) {
   if (int rc = pages::check_cache(c, "tree_attn", true, false)) return rc;
@@ -1462,8 +1648,8 @@ extern "C" int cab_tree_attn_fwd(const cab_page_cache* cache, int64_t layer, con
   for (const void* x : {p.k, p.v}) p.in_vec = p.in_vec && reinterpret_cast<uintptr_t>(x) % (4 * es) == 0;
   for (int i = 0; i < 3; ++i) p.in_vec = p.in_vec && p.ks[i] % 4 == 0 && p.vs[i] % 4 == 0;
   switch (cache->dtype) {
-    case CAB_DTYPE_F32: return launch_simt_d<float>(p, L.units, st);
-    case CAB_DTYPE_F16: return launch_simt_d<__half>(p, L.units, st);
-    default: return launch_simt_d<__nv_bfloat16>(p, L.units, st);
+    case CAB_DTYPE_F32: return launch_simt_d<float>(p, L, st);
+    case CAB_DTYPE_F16: return launch_simt_d<__half>(p, L, st);
+    default: return launch_simt_d<__nv_bfloat16>(p, L, st);
   }
 }

@@ -123,6 +123,13 @@ CASES = [
     (4, 4, 64, 20, 3, [100, 31], "chain", BF),
     (2, 1, 7, 1, 4, [33], "mask", FP),
     (2, 2, 128, 48, 2, [500, 3], "chain", BF),
+    # up to 8 rows on CUDA cores
+    (3, 1, 80, 24, 2, [100, 31, 0], "parents", HF),
+    (8, 1, 256, 16, 1, [700, 1], "chain", FP),
+    (4, 4, 8, 3, 7, [33, 400], "mask", FP),
+    (8, 8, 128, 48, 3, [500, 3], "parents", BF),
+    (1, 1, 64, 16, 1, [0, 31, 32, 3000], "chain", FP),
+    (2, 1, 128, 64, 1, [2000], "chain", FP),
 ]
 
 
@@ -196,7 +203,7 @@ def test_scores_that_grow_or_fall_along_the_cache(dtype, D, S, up):
     check(out, lse, q, [k.float().numpy()[None]], vs, [T], 1 / math.sqrt(D), dtype)
 
 
-@pytest.mark.parametrize("dtype,S,D", [(BF, 16, 128), (HF, 64, 64)])
+@pytest.mark.parametrize("dtype,S,D", [(BF, 16, 128), (HF, 64, 64), (FP, 16, 64)])
 def test_infinite_scores(dtype, S, D):
     """+inf among the seen scores gives NaN as softmax does; -inf is a weight of 0."""
     kp, vp, table, seq, ks, vs = build([300], 1, S, D, dtype)
@@ -244,11 +251,12 @@ def test_strides_rows_and_out(dtype, S, D):
     assert torch.equal(odd, out)
 
 
-@pytest.mark.parametrize("dtype,S,D,T", [(BF, 16, 128, 40), (HF, 64, 64, 12), (FP, 16, 64, 12), (BF, 16, 128, 150)])
-def test_what_is_not_seen_does_not_reach_the_output(dtype, S, D, T):
+@pytest.mark.parametrize("dtype,S,D,T,Hq", [(BF, 16, 128, 40, 4), (HF, 64, 64, 12, 4), (FP, 16, 64, 12, 4),
+                                            (BF, 16, 128, 150, 4), (FP, 16, 64, 7, 2)])
+def test_what_is_not_seen_does_not_reach_the_output(dtype, S, D, T, Hq):
     """Nodes with NaN or infinite keys and values change only the nodes that see them."""
     g = torch.Generator().manual_seed(9)
-    H, Hq, ctx = 2, 4, 100
+    H, ctx = 2, 100
     kp, vp, table, seq, ks, vs = build([ctx + T], H, S, D, dtype)
     q = torch.randn(1, Hq, T, D, generator=g).to(dtype).cuda()
     parents = random_parents(1, T, g, branch=0.3)
