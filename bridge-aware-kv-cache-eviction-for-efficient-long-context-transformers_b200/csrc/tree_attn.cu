@@ -62,6 +62,7 @@ struct Params {
   int32_t whole_units;  // no unit is cut: none can be longer than a few tiles
   int32_t in_vec;       // CUDA-core path: K / V rows can be read 4 elements at a time
   float *part_o, *part_ml;
+  int64_t* before;  // [n + 1] more than kScan sequences: the weight before each, for the join
 };
 
 struct Seq {
@@ -596,6 +597,7 @@ constexpr uint32_t kTmemO = 384;
 constexpr int kMaxShare = 4;
 constexpr int kLostRing = 16;  // tiles between the K loads and the softmax, at most kStages + 3
 constexpr int kUnitCost = 4;
+constexpr int kScan = 128;  // sequences up to which the join adds up the weights itself, before it waits
 constexpr int kWholeTiles = 4;  // rows of at most this many tiles are not cut: no join
 
 template <int D>
@@ -606,7 +608,7 @@ struct Cfg {
   // with as many stages as S / P buffers S(g) completed frees K stage g % 3, PV(g) V stage g % 3
   static constexpr bool kOneSignal = kStages == kBufs;
   static constexpr int kXchg = 2 * 2 * 128 * 4;  // references m [tile parity][row], sums [set][row]
-  static constexpr int kBars = (4 * kStages + 3 * kBufs + 4) * 8 + 32 + kLostRing;
+  static constexpr int kBars = (4 * kStages + 3 * kBufs + 6) * 8 + 32 + kLostRing;
   static constexpr int kBytes = (1 + 2 * kStages) * kTile + kXchg + kBars;
   static constexpr int kSmem = kBytes + 1024 < 232448 ? kBytes + 1024 : 232448;  // the kernel checks that it fits
   static_assert(kBytes <= 232448, "shared memory");
@@ -921,9 +923,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* s_full = v_empty + kStages;    // [3] S(g) is there
   uint64_t* p_full = s_full + kBufs;       // [3] P(g) is there (4 warps)
   uint64_t* buf_free = p_full + kBufs;     // [3] PV(g) has completed
-  uint64_t* q_full = buf_free + kBufs;     // Q of the segment is there
-  uint64_t* q_free = q_full + 1;           // the segment's products with Q have completed
-  uint64_t* drain = q_free + 1;            // [2]
+  uint64_t* q_full = buf_free + kBufs;     // [2] Q of the segment is there
+  uint64_t* q_free = q_full + 2;           // [2] the segment's products with Q have completed
+  uint64_t* drain = q_free + 2;            // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   int* odd_seg = abort_flag + 1;   // the last segment (from 1) whose V tiles held values that are not finite
@@ -945,7 +947,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 0) {
     // The barriers lie in one row: K / V stages, s_full (2: the product, and the issuer itself, which passes
     // on what the K loader wrote), p_full (4 warps), buf_free, q_full, q_free, drain; a lane each.
-    constexpr int kAll = 4 * kStages + 3 * kBufs + 4;
+    constexpr int kAll = 4 * kStages + 3 * kBufs + 6;
     for (int i = lane; i < kAll; i += 32) {
       const int j = i - 4 * kStages;
       mbar_init(&k_full[i], j < 0 ? 1 : j < kBufs ? 2 : j < 2 * kBufs ? 4 : 1);
@@ -978,6 +980,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   else asm volatile("barrier.cta.sync 14, %0;" ::"n"(kTcThreads) : "memory");
   tc_fence_after_sync();
   const uint32_t tmem = warp == 0 ? 0u : *tmem_slot;
+
+  // Up to 64 rows leave room for two Q buffers in the tile; the products read 128 rows from there all the
+  // same, and what lies behind a buffer's rows only reaches rows of S that nobody uses.
+  const uint32_t q_bufs = min(sh.nodes, p.T) * p.G <= 64 ? 2 : 1;
+  constexpr uint32_t kHalfQ = 64 * 128;
 
   Walk w;
   w.b = begin[0];
@@ -1023,22 +1030,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         return q < 0 || q >= p.pages ? -1 : q;  // -1: a page outside the pool
       };
       int e0 = page_of(0), e1 = page_of(1);  // read two tiles ahead
-      if (is_k) {
-        // Q, once the previous segment's last S, its reader, has completed (S runs ahead of the
-        // softmax, so the next segment's first S is done by the time the softmax gets there)
-        if (nq > 0) ok = mbar_wait(q_free, (nq - 1) & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+      // Q into its buffer once the buffer's last reader has completed: with two buffers the segment before
+      // the previous one, so Q is there ahead of its segment.
+      auto load_q = [&]() -> bool {
+        const uint32_t qb = nq & (q_bufs - 1), use = nq >> (q_bufs - 1);
         ++nq;
-        if (lane == 0) {
+        const bool got = __all_sync(0xffffffffu, mbar_wait(&q_free[qb], (use & 1) ^ 1, abort_flag));
+        if (got && lane == 0) {
           const int nodes = min(sh.nodes, p.T);
-          mbar_arrive_expect_tx(q_full, nodes * p.G * D * 2);
+          mbar_arrive_expect_tx(&q_full[qb], nodes * p.G * D * 2);
 #pragma unroll
           for (int k = 0; k < C::kAtoms; ++k)
-            tma_load_5d(sQ + k * 16384, &qmap, q_full, 64 * k, 0, (w.set * sh.wide + side) * sh.nodes, w.hk, w.b);
+            tma_load_5d(sQ + qb * kHalfQ + k * 16384, &qmap, &q_full[qb], 64 * k, 0, (w.set * sh.wide + side) * sh.nodes, w.hk, w.b);
         }
         __syncwarp();
-      }
+        return got;
+      };
+      if (is_k) ok = load_q();
+      if (!ok) break;
       for (int i = 0; i < T; ++i, ++g) {
         const int e2 = page_of(i + 2);
         const uint32_t st = g % kStages;
@@ -1062,22 +1071,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     if (!ok) {  // copies still in flight land before the CTA ends
       for (uint32_t k = 1; k <= kStages && k <= g; ++k) (void)mbar_wait(&full[(g - k) % kStages], ((g - k) / kStages) & 1, nullptr);
-      if (nq > 0) (void)mbar_wait(q_full, (nq - 1) & 1, nullptr);
+      for (uint32_t k = 1; k <= q_bufs && k <= nq; ++k) (void)mbar_wait(&q_full[(nq - k) % q_bufs], (nq - k) / q_bufs & 1, nullptr);
     }
     __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------------- S = Q K^T
     if (lane == 0) {
       constexpr uint32_t idesc = make_idesc_f16(128, 128, kBF16 ? 1 : 0, 0, 0);
-      const uint64_t dq = make_smem_desc(smem_u32(sQ), 16, 1024, 2);
+      const uint64_t dQ = make_smem_desc(smem_u32(sQ), 16, 1024, 2);
       const uint64_t dK = make_smem_desc(smem_u32(sK), 16, 1024, 2);
       uint32_t g = 0, seg = 0;
       bool ok = true;
       for (; w.left > 0 && ok; walk_next(p, sh, w)) {
         const int T = segment_of(p, sh, w, w.set * sh.wide + side).count;
         if (T == 0) continue;
-        if (!mbar_wait(q_full, seg & 1, abort_flag)) break;
+        const uint32_t qb = seg & (q_bufs - 1);
+        if (!mbar_wait(&q_full[qb], seg >> (q_bufs - 1) & 1, abort_flag)) break;
         ++seg;
+        const uint64_t dq = dQ + static_cast<uint64_t>(qb * (kHalfQ >> 4));
         for (int i = 0; i < T; ++i, ++g) {
           const uint32_t st = g % kStages, buf = g % kBufs;
           if (!mbar_wait(&k_full[st], (g / kStages) & 1, abort_flag) ||
@@ -1096,7 +1107,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           mma_commit(&s_full[buf]);
           mbar_arrive(&s_full[buf]);
         }
-        mma_commit(q_free);
+        mma_commit(&q_free[qb]);
       }
       mma_commit(&drain[0]);
       (void)mbar_wait(&drain[0], 0, nullptr);
@@ -1104,6 +1115,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncwarp();
   } else if (warp == 2) {
     // ---------------------------------------------------------------- O += P V
+    if (p.n > kScan && blockIdx.x == 0 && !p.whole_units) {  // while the first tiles are on their way
+      int64_t base = 0;
+      for (int b0 = 0; b0 < p.n; b0 += 32) {
+        const int b = b0 + lane;
+        int64_t inc = b < p.n ? static_cast<int64_t>(head_weight(p, sh, load_seq(p, b))) * p.Hkv : 0;
+        const int64_t own = inc;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += u;
+        }
+        if (b < p.n) p.before[b] = base + inc - own;
+        base += __shfl_sync(0xffffffffu, inc, 31);
+      }
+      if (lane == 0) p.before[p.n] = base;
+      __syncwarp();
+    }
     if (lane == 0) {
       constexpr uint32_t idesc = make_idesc_f16(128, D, kBF16 ? 1 : 0, 0, 1);
       const uint64_t dV = make_smem_desc(smem_u32(sV), 16384, 1024, 2);
@@ -1222,7 +1250,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           l += weights<kBF16>(s, p.scale_log2, sub, t_s);
           load_half(1);
           l += weights<kBF16>(s, p.scale_log2, sub, t_s + 32);
-          const bool grown = m_prev != -INFINITY && m_new != m_prev;
+          const bool grown = live && m_prev != -INFINITY && m_new != m_prev;  // rows past the last hold anything
           if (__any_sync(0xffffffffu, grown)) {
             // PV(g - 1) has completed: its barrier's phase before, PV(g - 4), was needed by S(g - 1)
             (void)mbar_wait(&buf_free[(g - 1) % kBufs], ((g - 1) / kBufs) & 1, abort_flag);
@@ -1338,17 +1366,23 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ Param
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int grp = blockIdx.x % sh.groups, hk = blockIdx.x / sh.groups % p.Hkv, b = blockIdx.x / sh.groups / p.Hkv;
   const int set = grp / sh.wide, side = grp % sh.wide;
+  if (p.n > kScan) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (warp == 0) {
     int64_t total = 0, before = 0;
-    for (int i = lane; i < p.n; i += 32) {
-      const int64_t x = static_cast<int64_t>(head_weight(p, sh, load_seq(p, i))) * p.Hkv;
-      total += x;
-      if (i < b) before += x;
-    }
+    if (p.n > kScan) {
+      total = p.before[p.n];
+      before = p.before[b];
+    } else {
+      for (int i = lane; i < p.n; i += 32) {
+        const int64_t x = static_cast<int64_t>(head_weight(p, sh, load_seq(p, i))) * p.Hkv;
+        total += x;
+        if (i < b) before += x;
+      }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      total += __shfl_xor_sync(0xffffffffu, total, o);
-      before += __shfl_xor_sync(0xffffffffu, before, o);
+      for (int o = 16; o; o >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+      }
     }
     const Seq s = load_seq(p, b);
     before += static_cast<int64_t>(hk) * head_weight(p, sh, s);
@@ -1426,7 +1460,7 @@ struct Layout {
   bool tc, whole;
   int splits, part_rows, ctas, rows;
   int64_t units;
-  size_t part_o, part_ml, total;
+  size_t part_o, part_ml, before, total;
 };
 
 inline bool use_tensor_cores(const cab_page_cache* c, int64_t G) {
@@ -1454,7 +1488,8 @@ inline Layout layout(const cab_page_cache* c, int64_t n, int64_t Hq, int64_t T) 
     if (L.whole) return L;
     const size_t slots = static_cast<size_t>(L.ctas) * 2 * L.part_rows;
     L.part_ml = slots * D * 4;
-    L.total = L.part_ml + slots * 8;
+    L.before = (L.part_ml + slots * 8 + 15) & ~size_t(15);
+    L.total = L.before + (n > kScan ? static_cast<size_t>(n + 1) * 8 : 0);
     return L;
   }
   L.rows = simt_rows(c, R);
@@ -1584,6 +1619,11 @@ extern "C" int cab_tree_attn_fwd(const cab_page_cache* cache, int64_t layer, con
   if (L.total > 0 && (!workspace || workspace_bytes < L.total))
     return fail(CAB_ERR_WORKSPACE, "tree_attn: workspace of %zu bytes needed, %zu given", L.total, workspace_bytes);
   if (L.total > 0 && !aligned16(workspace)) return fail(CAB_ERR_INVALID_ARG, "tree_attn: workspace must be 16-byte aligned");
+  if (L.tc) {  // what the ranges count in 32 bits
+    const Share sh = share_of(static_cast<int>(Hq / cache->heads), static_cast<int>(T));
+    if (cache->heads * sh.sets * (cache->width * cache->page_size / 128 + 1 + kUnitCost) >= (int64_t)1 << 31)
+      return fail(CAB_ERR_UNSUPPORTED, "tree_attn: more than 2^31 tiles a sequence");
+  }
   if (L.units >= (int64_t)1 << 31) return fail(CAB_ERR_UNSUPPORTED, "tree_attn: too many row tiles");
   const int64_t es = static_cast<int64_t>(dtype_size(cache->dtype));
   Params p{};
@@ -1622,6 +1662,7 @@ extern "C" int cab_tree_attn_fwd(const cab_page_cache* cache, int64_t layer, con
   if (L.total > 0) {
     p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + L.part_o);
     p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + L.part_ml);
+    p.before = reinterpret_cast<int64_t*>(static_cast<uint8_t*>(workspace) + L.before);
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (L.tc) {
