@@ -163,6 +163,11 @@ SHAPES = [
     (1, 1, 128, 128, 2, [70001], 0, BF),
     (2, 1, 64, 16, 6, [40003, 3], 4096, HF),
     (4, 1, 64, 16, 700, [10], 0, BF),           # 2800 rows of a KV head: several sets of groups
+    # more than 128 sequences whose rows are cut between CTAs
+    (4, 2, 64, 16, 2, [53 * i % 120 + 2500 * (i % 50 == 7) for i in range(150)], 0, BF),
+    (2, 1, 128, 32, 70, [3100] + [i % 3 for i in range(128)], 0, HF),
+    (1, 1, 64, 64, 1, [0] * 299 + [6000], 0, BF),
+    (8, 2, 64, 16, 40, [31 * i % 200 for i in range(257)], 64, BF),   # 160 rows a KV head, a pair of groups
 ]
 
 
