@@ -588,8 +588,11 @@ __global__ void __launch_bounds__(kSimtThreads) simt_join_kernel(const __grid_co
 // lowers the clock to 1.3 - 1.6 GHz; 1.08 GB from HBM, so the CTAs side by side share each tile through L2.
 // Before that: one tile a time on two streams with an O each 407 us; 64 keys a thread 361 us.
 //
-// Every mbarrier has one waiter per phase and direction, or its next phase needs the waiter's own
-// next step, so parity waits never meet a barrier two phases on.
+// A parity wait must not meet a barrier two phases away from its own. Each loader and issuer waits for every phase
+// of its barriers in turn. A softmax set skips the other set's tiles; what ties it to them is the hand-over of m,
+// and between segments the meeting over O (rows that are nodes) or over the cleaned V (every live group's last
+// tile holds its own nodes, so only a range's last segment has no such meeting). A group without a node would
+// have neither, so it takes no tiles at all: its rows' zeros are written straight away.
 
 constexpr int kTcThreads = 384;  // warps 0 / 3: K / V loads, 1: S, 2: PV, 4-11: softmax and epilogue
 constexpr float kRescaleThreshold = 8.0f;
@@ -668,16 +671,18 @@ __device__ __forceinline__ void walk_next(const Params& p, const Share& sh, Walk
   }
   w.tiles = unit_tiles(p, sh, w.s, w.set);
 }
-// The walk's segment: group grp's tiles [first, first + count) (the unit's longest group has them all).
+// The walk's segment: group grp's tiles [first, first + count) (the unit's longest group has them all). A group
+// without a node has no tiles to compute, and `zeros` where its one place in the list is in the range.
 struct Segment {
   int first, count;
+  bool zeros;
 };
 __device__ __forceinline__ Segment segment_of(const Params& p, const Share& sh, const Walk& w, int grp) {
-  if (grp >= sh.groups) return Segment{0, 0};
-  const int own = min(w.tiles, tiles_of(group_keys(p, sh, w.s, grp, grp)));
-  if (p.whole_units) return Segment{0, own};
-  const int first = max(0, w.at - kUnitCost), end = min(own, w.at + w.left - kUnitCost);
-  return Segment{first, max(0, end - first)};
+  if (grp >= sh.groups) return Segment{0, 0, false};
+  const int keys = group_keys(p, sh, w.s, grp, grp), own = min(w.tiles, tiles_of(keys));
+  const int first = p.whole_units ? 0 : max(0, w.at - kUnitCost);
+  const int end = p.whole_units ? own : min(own, w.at + w.left - kUnitCost), count = max(0, end - first);
+  return keys > 0 ? Segment{first, count, false} : Segment{0, 0, count > 0};
 }
 
 // Where range c starts. (A 64-bit division takes several hundred clocks, a 32-bit one about a hundred.)
@@ -1177,10 +1182,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int grp = w.set * sh.wide + side;
       const Segment sg = segment_of(p, sh, w, grp);
       const int T = sg.count;
+      const int t = grp * sh.nodes + r / p.G, rows = min(sh.nodes, p.T - grp * sh.nodes) * p.G;
+      if (sg.zeros && r < rows) {  // no row of the group is a node; the row's two threads take half the columns each
+        const int h = w.hk * p.G + r % p.G;
+        InT* orow = static_cast<InT*>(p.out) + w.b * p.os[0] + h * p.os[1] + t * p.os[2] + kb * (D / 2);
+        if (p.out_vec) {
+#pragma unroll
+          for (int c = 0; c < D / 2; c += 8) *reinterpret_cast<uint4*>(orow + c) = make_uint4(0u, 0u, 0u, 0u);
+        } else {
+          for (int c = 0; c < D / 2; ++c) orow[c] = from_f32<InT>(0.f);
+        }
+        if (p.lse && kb == 0) p.lse[(static_cast<int64_t>(w.b) * p.Hq + h) * p.T + t] = -INFINITY;
+      }
       if (T == 0) continue;
       ++seg;
       const Seq q = w.s;
-      const int t = grp * sh.nodes + r / p.G, rows = min(sh.nodes, p.T - grp * sh.nodes) * p.G;
       const bool live = r < rows && t < q.m;
       const bool any_live = __any_sync(0xffffffffu, live);
       const int key_lo = sg.first * 128, keys = group_keys(p, sh, q, grp, grp);
@@ -1190,7 +1206,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t g = g0 + i, buf = g % kBufs;
         const uint32_t t_s = tmem + lanes + buf * 128;  // S in, P out
         const int key0 = key_lo + i * 128;
-        // tiles between this set's were S before this one, so the barrier is at most this phase behind
+        // S(g - 3) has completed: this set, or the other before they last met, waited for it or for a later tile
         (void)mbar_wait(&s_full[buf], (g / kBufs) & 1, abort_flag);
         tc_fence_after_sync();
         const bool bad = *reinterpret_cast<volatile uint8_t*>(&lost[g % kLostRing]) != 0;
