@@ -948,7 +948,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const Share sh = share_of(p.G, p.T);
   const int range = blockIdx.x / sh.wide, side = blockIdx.x % sh.wide;
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 0) {
     // The barriers lie in one row: K / V stages, s_full (2: the product, and the issuer itself, which passes
     // on what the K loader wrote), p_full (4 warps), buf_free, q_full, q_free, drain; a lane each.
@@ -970,6 +969,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   if (warp == 2) tmem_alloc(tmem_slot, 512);
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the inputs of this call may be the kernel before's results
+  // Only now, with the kernel before complete, may the join start: it reads the lengths before its own wait.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 0) {
     __syncwarp();
     const Begin x = find_range(p, sh, range, gridDim.x / sh.wide);
@@ -1373,7 +1374,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 2) tmem_dealloc(tmem, 512);
 }
 
-// Adds a cut unit's partial sums: one warp per row, in key order.
+// Adds a cut unit's partial sums: one warp per row, in key order. Up to kScan sequences the search for the unit
+// reads lens, rows and nodes ahead of the wait for tc_kernel, which is sound because tc_kernel lets this kernel
+// start only after its own wait: whatever wrote them has completed by then.
 template <int D, bool kBF16>
 __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ Params p, int ctas_max) {
   using InT = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
