@@ -933,8 +933,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* drain = q_free + 2;            // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  int* odd_seg = abort_flag + 1;   // the last segment (from 1) whose V tiles held values that are not finite
-  int* begin = odd_seg + 1;        // the range: first sequence, weight before it in there, own weight
+  int* odd = abort_flag + 1;       // [2] the last odd / even tail segment (from 1) with values of nodes that are not finite
+  int* begin = odd + 2;            // the range: first sequence, weight before it in there, own weight
   uint8_t* lost = reinterpret_cast<uint8_t*>(begin + 3);  // [kLostRing] tile has a page outside the pool
   {
     uint32_t dyn;
@@ -958,7 +958,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     if (lane == 0) {
       *abort_flag = 0;
-      *odd_seg = 0;
+      odd[0] = odd[1] = 0;
     }
     fence_barrier_init();
   }
@@ -1178,7 +1178,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t t_o = tmem + lanes + kTmemO;
     float *ref = xchg, *sums = xchg + 256;
     uint32_t g0 = 0;  // tiles of earlier segments
-    int seg = 0;
+    // Segments that reach into their nodes. A warp that sets odd[] for tail segment x + 2 has met the others in
+    // x + 1, so all of them have read it for x: two words, by the segment's parity.
+    int tails = 0;
     for (; w.left > 0; walk_next(p, sh, w)) {
       const int grp = w.set * sh.wide + side;
       const Segment sg = segment_of(p, sh, w, grp);
@@ -1196,12 +1198,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (p.lse && kb == 0) p.lse[(static_cast<int64_t>(w.b) * p.Hq + h) * p.T + t] = -INFINITY;
       }
       if (T == 0) continue;
-      ++seg;
       const Seq q = w.s;
       const bool live = r < rows && t < q.m;
       const bool any_live = __any_sync(0xffffffffu, live);
       const int key_lo = sg.first * 128, keys = group_keys(p, sh, q, grp, grp);
       const bool has_tail = key_lo + T * 128 > q.ctx;
+      tails += has_tail;
       float m_run = -INFINITY, l = 0.f;  // this set's sum, relative to its last m
       for (int i = kb; i < T; i += 2) {
         const uint32_t g = g0 + i, buf = g % kBufs;
@@ -1220,7 +1222,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const uint32_t st = g % kStages;
           (void)mbar_wait(&v_full[st], (g / kStages) & 1, abort_flag);
           if (key0 + r >= q.ctx) {
-            if (clean_v_row<D, kBF16>(sV + st * C::kTile, r, key0 + r, q)) *reinterpret_cast<volatile int*>(odd_seg) = seg;
+            if (clean_v_row<D, kBF16>(sV + st * C::kTile, r, key0 + r, q)) *reinterpret_cast<volatile int*>(&odd[tails & 1]) = tails;
             fence_proxy_async_smem();
           }
           if (live) see = seen_bits(p, q, w.b, t, key0, bad);
@@ -1308,7 +1310,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (has_tail) softmax_sync();  // all warps have cleaned their part of V
       if (quad * 32 < rows) {
-        const bool odd = has_tail && *reinterpret_cast<volatile int*>(odd_seg) == seg;
+        const bool mend = has_tail && *reinterpret_cast<volatile int*>(&odd[tails & 1]) == tails;
         const bool whole = T == tiles_of(keys);
         const float inv = live && l != 0.f ? 1.f / l : 0.f;
         const int h = w.hk * p.G + r % p.G;
@@ -1323,7 +1325,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tmem_wait_ld();
           }
           if (r >= rows) continue;
-          if (odd && live) {
+          if (mend && live) {
             float more[32];  // rare: kept out of the sum's registers
 #pragma unroll
             for (int k = 0; k < 32; ++k) more[k] = 0.f;

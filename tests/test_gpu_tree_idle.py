@@ -70,3 +70,28 @@ def test_zeros_into_an_output_off_16_bytes(D):
     _, lse = tree_attention(q.cuda(), kp, vp, table, seq, num_nodes=nodes, out=out, return_lse=True)
     check(out, lse, q, ks, vs, [0, 3, 0], 1 / math.sqrt(D), BF)
     assert (out[::2] == 0).all() and (hold[1:].view(3, 4, 3, D + 3)[..., D:] == 7.0).all() and float(hold[0]) == 7.0
+
+
+@pytest.mark.parametrize("D,S,T,Hq,dtype", [(64, 16, 1, 8, HF), (128, 16, 1, 8, BF), (128, 16, 7, 24, BF), (64, 64, 3, 40, HF)])
+@pytest.mark.parametrize("table_tokens", [0, 2048])
+def test_infinite_values_of_nodes_in_many_short_rows(D, S, T, Hq, dtype, table_tokens):
+    """Many units after one another in a CTA, every other one with infinite values at its nodes: each row gets its
+    own nodes' infinities, in every run."""
+    n, H = 400, 8
+    lens = [T + 3 * i % 120 for i in range(n)]
+    kp, vp, table, seq, _, _ = build(lens, H, S, D, dtype)
+    if table_tokens:
+        table = torch.nn.functional.pad(table, (0, table_tokens // S - table.shape[1]), value=-1)
+    q = torch.randn(n, Hq, T, D).to(dtype).cuda()
+    odd = torch.arange(1, n, 2)
+    for i in odd.tolist():
+        x = lens[i] - T  # node 0: every node sees it
+        vp[int(table[i, x // S]), :, x % S, 5::16] = math.inf
+        vp[int(table[i, x // S]), :, x % S, 9::16] = -math.inf
+    first = tree_attention(q, kp, vp, table, seq)
+    for i, got in ((odd, first[odd.cuda()]), (odd - 1, first[odd.cuda() - 1])):
+        hit = bool(i[0] % 2)
+        assert ((got[..., 5::16] == math.inf) == hit).all() and ((got[..., 9::16] == -math.inf) == hit).all()
+        assert torch.isfinite(got[..., 0::16]).all()
+    for _ in range(20):
+        assert torch.equal(tree_attention(q, kp, vp, table, seq), first)
