@@ -62,6 +62,7 @@ __device__ __forceinline__ void cluster_sync(int nc) {
     __syncthreads();
     return;
   }
+  __syncwarp();  // the aligned form wants the whole warp
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The shared-memory word `p` of CTA `rank` of the cluster.

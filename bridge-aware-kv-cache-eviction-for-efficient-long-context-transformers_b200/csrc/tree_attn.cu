@@ -1227,6 +1227,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           if (live) see = seen_bits(p, q, w.b, t, key0, bad);
         }
+        __syncwarp();  // waits and masks end lane by lane; the TMEM loads want the whole warp
         if (any_live) {
           uint32_t s[64];
           auto load_half = [&](int h) {
@@ -1266,6 +1267,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (m_run != m_new) l *= ex2(m_run - m_new);  // from -inf: l is 0
           m_run = m_new;
           const float sub = m_new == -INFINITY ? 0.f : m_new;  // nothing above -inf so far: weights 0
+          __syncwarp();
           l += weights<kBF16>(s, p.scale_log2, sub, t_s);
           load_half(1);
           l += weights<kBF16>(s, p.scale_log2, sub, t_s + 32);
@@ -1273,6 +1275,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (__any_sync(0xffffffffu, grown)) {
             // PV(g - 1) has completed: its barrier's phase before, PV(g - 4), was needed by S(g - 1)
             (void)mbar_wait(&buf_free[(g - 1) % kBufs], ((g - 1) / kBufs) & 1, abort_flag);
+            __syncwarp();
             tc_fence_after_sync();
             const float alpha = grown ? ex2(m_prev - m_new) : 1.f;
 #pragma unroll 1
@@ -1320,6 +1323,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int c = 0; c < D / 2; c += 32) {
           uint32_t x[32];
+          __syncwarp();  // from the meetings, or from the columns before
           if (any_live) {
             tmem_ld32(t_o + kb * (D / 2) + c, x);
             tmem_wait_ld();

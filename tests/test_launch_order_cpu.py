@@ -29,3 +29,16 @@ def test_every_kernel_launched_behind_another_waits_for_it():
     for name in ("tree_attn.cu", "paged_cache.cu"):
         for kernel, body in kernels(name).items():
             assert "griddepcontrol.wait" in body or "grid_dependency_wait()" in body, kernel
+
+
+def test_warps_are_whole_at_instructions_that_want_them_whole():
+    """TMEM loads and the cluster barrier are `.aligned`: behind waits, masks and an early `continue`, which lanes
+    leave one by one, a __syncwarp() comes first."""
+    tc = kernels("tree_attn.cu")["tc_kernel"]
+    for start in ("if (masked) {", "take_over(quad", "for (int c = 0; c < D / 2; c += 32) {"):
+        part = tc[tc.index(start):]
+        first = min(part.find(x) for x in ("tmem_ld32(", "weights<") if x in part)
+        assert "__syncwarp()" in part[:first], start
+    update = re.sub(r"//[^\n]*", "", (CSRC / "paged_cache.cu").read_text())
+    sync = update[update.index("void cluster_sync("):]
+    assert "__syncwarp()" in sync[:sync.index(".aligned")]
