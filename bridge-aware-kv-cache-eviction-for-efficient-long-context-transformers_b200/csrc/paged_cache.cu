@@ -25,6 +25,7 @@
 #include "cab_ptx.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace cab {
 namespace pages {
@@ -627,6 +628,24 @@ void launch_after(void (*kernel)(Args...), dim3 grid, int threads, cudaStream_t 
   cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Raises a kernel's limit of dynamic shared memory, once per device and to the most that any call needs: the limit
+// is the device's, not the thread's, so a limit set per call could be lowered by another thread before the launch.
+template <auto Kernel>
+int allow_smem(size_t most, const char* what) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return CAB_OK;
+  const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail(CAB_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
+  }
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return CAB_OK;
+}
+
 inline int check_cache(const cab_page_cache* c, const char* what, bool data, bool state = true) {
   if (!c) return fail(CAB_ERR_INVALID_ARG, "%s: NULL cache", what);
   if (!c->block_table || !c->seq_lens || (state && (!c->ref_counts || !c->status)))
@@ -741,10 +760,9 @@ extern "C" int cab_pages_update(const cab_page_cache* cache, const int32_t* src,
   p.div_mul = static_cast<uint32_t>((((uint64_t)1 << (31 + log2s)) + cache->page_size - 1) / cache->page_size);
   p.div_shift = 31 + log2s;
 
-  const int64_t words = (cache->rows + 31) / 32;
-  const size_t smem = static_cast<size_t>(15 * n + 1 + 3 * words) * 4;
-  if (smem > 40 * 1024)
-    cudaFuncSetAttribute(update_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  auto smem_of = [](int64_t pairs, int64_t rows) { return static_cast<size_t>(15 * pairs + 1 + 3 * ((rows + 31) / 32)) * 4; };
+  const size_t smem = smem_of(n, cache->rows);
+  if (int rc = allow_smem<update_kernel>(smem_of(kMaxPairs, kMaxRows), "pages update_kernel")) return rc;
   // one CTA reads up to 8 values a thread of each array in one go; more are spread over a cluster
   const int64_t ints = std::max(cache->pages, n * std::max(cache->width, keep_cols));
   launch_after(update_kernel, dim3(ints > 8 * kUpdateThreads ? kMaxCluster : 1), kUpdateThreads, static_cast<cudaStream_t>(stream), smem,

@@ -18,7 +18,6 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -1551,13 +1550,7 @@ template <int D, bool kBF16>
 int launch_tc(const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& qm, const Params& p, const Layout& L,
               cudaStream_t st) {
   using C = Cfg<D>;
-  static std::atomic<uint64_t> ready{0};  // devices on which the kernel has been set up
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1u)) {
-    cudaFuncSetAttribute(tc_kernel<D, kBF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-    if (dev >= 0 && dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
-  }
+  if (int rc = pages::allow_smem<tc_kernel<D, kBF16>>(C::kSmem, "tree_attn tc_kernel")) return rc;
   pages::launch_after(tc_kernel<D, kBF16>, dim3(L.ctas), kTcThreads, st, C::kSmem, 1, km, vm, qm, p);
   if (int rc = check_launch("tree_attn tc_kernel")) return rc;
   if (L.whole) return CAB_OK;
@@ -1571,9 +1564,9 @@ int launch_tc(const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& q
 
 template <typename T, int DC, int RW>
 int launch_simt(const Params& p, int64_t units, cudaStream_t st) {
-  const int Dp = (p.D + 3) & ~3;
-  const size_t smem = static_cast<size_t>(4 * RW * (Dp + 32) + kKeysTile * (Dp + 4) + kKeysTile * Dp) * 4;
-  if (smem > 48 * 1024) cudaFuncSetAttribute(simt_kernel<T, DC, RW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  auto smem_of = [](int Dp) { return static_cast<size_t>(4 * RW * (Dp + 32) + kKeysTile * (Dp + 4) + kKeysTile * Dp) * 4; };
+  const size_t smem = smem_of((p.D + 3) & ~3);
+  if (int rc = pages::allow_smem<simt_kernel<T, DC, RW>>(smem_of(32 * DC), "tree_attn simt_kernel")) return rc;
   pages::launch_after(simt_kernel<T, DC, RW>, dim3(static_cast<unsigned>(units), static_cast<unsigned>(p.splits)), kSimtThreads, st, smem, 1, p);
   if (int rc = check_launch("tree_attn simt_kernel")) return rc;
   if (p.splits == 1) return CAB_OK;
