@@ -728,6 +728,8 @@ extern "C" int cab_pages_update(const cab_page_cache* cache, const int32_t* src,
   if (n * keep_cols >= (int64_t)1 << 31) return fail(CAB_ERR_UNSUPPORTED, "pages_update: more than 2^31 list entries a call");
   if (keep_cols > 0 && (!keep || (keep_bytes != 4 && keep_bytes != 8))) return fail(CAB_ERR_INVALID_ARG, "pages_update: keep must be int32 or int64");
   if (keep_cols > 0 && !copies) return fail(CAB_ERR_INVALID_ARG, "pages_update: a keep list needs copies");
+  // the snapshot of the source rows, which other rows are made from, is taken for the copies alone
+  if (dst && !copies) return fail(CAB_ERR_INVALID_ARG, "pages_update: rows that become others need copies");
   if (grow_value < 0) return fail(CAB_ERR_INVALID_ARG, "pages_update: negative growth");
   const UpdateLayout L = update_layout(cache, n);
   if (!workspace || workspace_bytes < L.total)

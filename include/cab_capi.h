@@ -361,8 +361,8 @@ CAB_API int cab_pages_update_workspace_size(const cab_page_cache* cache, int64_t
  * Arrays may be NULL: src (0 .. n-1), dst (src), start (start_value; < 0: the whole length),
  * keep_num (keep_cols), grow (grow_value). keep is int32 or int64 (keep_bytes 4 or 8), any
  * order; keep_num has a stride. A row may be written once per call; n <= 1024.
- * copies == 0: for calls that only lengthen rows or free them: no list, and no last page may
- * need a copy (k_pages / v_pages are not touched). All or nothing: on a device-side refusal
+ * copies == 0: for calls that only lengthen rows or free them: no list, dst NULL, and no last page
+ * may need a copy (k_pages / v_pages are not touched). All or nothing: on a device-side refusal
  * only the status word changes.
  * Applies the eviction that CABCache._evict makes (cab_attention/cache/cab_cache.py:177-226).
  */
