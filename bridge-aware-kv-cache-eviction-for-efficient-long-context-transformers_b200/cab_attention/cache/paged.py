@@ -32,6 +32,7 @@ STATUS = {1: "not enough free pages", 2: "a row would hold more tokens than its 
           4: "a row outside the table, or named twice as a destination",
           8: "a length, count or kept position out of range",
           16: "a table entry outside the pages, or a partly filled page that two rows share"}
+MAX_COUNT = 2 ** 31 - 1  # larger than any row: the device refuses it, and it does not wrap around on the way
 
 
 class PagedKVCache:
@@ -70,11 +71,11 @@ class PagedKVCache:
         if isinstance(start, torch.Tensor):
             start = int32_vector(start, n, "start", self.device)
         else:
-            start_value, start = (-1 if start is None else int(start)), None
+            start_value, start = (-1 if start is None else min(int(start), MAX_COUNT)), None
         if isinstance(grow, torch.Tensor):
             grow = int32_vector(grow, n, "num_new", self.device)
         else:
-            grow_value, grow = int(grow), None
+            grow_value, grow = min(int(grow), MAX_COUNT), None
         L = _lib.lib()
         size = self._sizes.get(n)
         if size is None:

@@ -749,7 +749,7 @@ extern "C" int cab_pages_update(const cab_page_cache* cache, const int32_t* src,
   p.keep_num = keep_cols > 0 ? keep_num : nullptr;
   p.keep_num_stride = keep_num_stride;
   p.grow = grow;
-  p.grow_value = grow_value;
+  p.grow_value = std::min(grow_value, (int64_t)INT32_MAX);  // more than any row has room for; sums stay in 64 bits
   p.n = static_cast<int32_t>(n);
   p.copies = copies != 0;
   p.header = reinterpret_cast<int32_t*>(ws);

@@ -77,3 +77,21 @@ def test_a_write_after_a_refusal_does_nothing(T):
     same(c, o)
     c.write(0, kv, kv, rows=dev([-1]))  # the refusal that was there stays the only one
     same(c, o)
+
+
+def test_counts_that_do_not_fit():
+    """Numbers past 31, 32, 63 and 64 bits are refused like any count that is too large."""
+    c, _ = make(P=20, R=3, W=6)
+    c.extend(dev([40, 16, 0]))
+    c.check()
+    o = oracle_of(c)
+    for big in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, 2 ** 63 - 1, 2 ** 63, 2 ** 64 + 1, 10 ** 30):
+        for call, bit in ((lambda: c.extend(big), 2), (lambda: c.extend(big, dev([1])), 2),
+                          (lambda: c.truncate(big), 8),
+                          (lambda: c.compact(dev([[0]]), start=big, src=dev([0])), 8)):
+            call()
+            o.status = bit
+            same(c, o)
+            with pytest.raises(RuntimeError, match="paged KV cache"):
+                c.check()
+            o.status = 0
