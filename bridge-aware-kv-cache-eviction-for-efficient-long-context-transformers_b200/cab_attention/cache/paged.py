@@ -87,8 +87,8 @@ class PagedKVCache:
         keep_bytes = keep_stride = keep_cols = num_stride = 0
         if keep is not None:
             keep_ptr, keep_bytes, keep_stride, keep_cols = keep.data_ptr(), keep.element_size(), keep.stride(0), keep.shape[1]
-            if keep_num is not None:
-                num_ptr, num_stride = keep_num.data_ptr(), keep_num.stride(0)
+        if keep_num is not None:
+            num_ptr, num_stride = keep_num.data_ptr(), keep_num.stride(0)
         call_on(self.device, "cab_pages_update", L.cab_pages_update, self._c, None if src is None else src.data_ptr(),
                 None if dst is None else dst.data_ptr(), n, None if start is None else start.data_ptr(), start_value,
                 keep_ptr, keep_bytes, keep_stride, keep_cols, num_ptr, num_stride,

@@ -746,7 +746,7 @@ extern "C" int cab_pages_update(const cab_page_cache* cache, const int32_t* src,
   p.keep64 = keep_bytes == 8;
   p.keep_stride = keep_stride;
   p.keep_cols = keep_cols;
-  p.keep_num = keep_cols > 0 ? keep_num : nullptr;
+  p.keep_num = keep_num;  // without a list, counts other than 0 are refused
   p.keep_num_stride = keep_num_stride;
   p.grow = grow;
   p.grow_value = std::min(grow_value, (int64_t)INT32_MAX);  // more than any row has room for; sums stay in 64 bits

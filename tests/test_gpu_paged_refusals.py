@@ -95,3 +95,21 @@ def test_counts_that_do_not_fit():
             with pytest.raises(RuntimeError, match="paged KV cache"):
                 c.check()
             o.status = 0
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_counts_of_an_empty_list(dtype):
+    """A keep list without columns holds no positions, whatever keep_num says."""
+    c, _ = make(P=20, R=3, W=6)
+    c.extend(dev([40, 16, 5]))
+    o = oracle_of(c)
+    empty = torch.empty(2, 0, dtype=dtype, device="cuda")
+    c.compact(empty, dev([0, 2]), start=7, src=dev([0, 1]))
+    o.status = 8
+    same(c, o)
+    with pytest.raises(RuntimeError, match="paged KV cache"):
+        c.check()
+    c.compact(empty, dev([0, 0]), start=7, src=dev([0, 1]))
+    c.compact(empty[:1], start=3, src=dev([2]))
+    c.check()
+    assert c.seq_lens.tolist() == [7, 7, 3]
