@@ -26,6 +26,7 @@ namespace tree {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int64_t kMaxTokens = 0x7fffffff - 512;  // of a row: positions up to two 128-key tiles past it fit 32 bits
 constexpr int kMaxTree = 1024;  // nodes of a tree given by parents: a query walks up its ancestors
 
 __device__ __forceinline__ float ex2(float x) {
@@ -1600,6 +1601,8 @@ inline int check_sizes(const cab_page_cache* c, int64_t n, int64_t Hq, int64_t T
   if (int rc = pages::check_cache(c, "tree_attn", true, false)) return rc;
   if (n <= 0 || Hq <= 0 || T <= 0) return fail(CAB_ERR_INVALID_ARG, "tree_attn: non-positive size");
   if (Hq % c->heads != 0) return fail(CAB_ERR_INVALID_ARG, "tree_attn: Hq %% Hkv != 0");
+  if (c->width * c->page_size > kMaxTokens)
+    return fail(CAB_ERR_UNSUPPORTED, "tree_attn: table rows for more than %lld tokens", (long long)kMaxTokens);
   if (c->dim > 256) return fail(CAB_ERR_UNSUPPORTED, "tree_attn: head_dim %lld (at most 256)", (long long)c->dim);
   if (n > pages::kMaxRows || Hq > 65536 || T > 65536 || n * Hq * T >= (int64_t)1 << 31)
     return fail(CAB_ERR_UNSUPPORTED, "tree_attn: more than 2^31 rows, or a size above 65536");

@@ -398,7 +398,8 @@ CAB_API int cab_tree_attn_workspace_size(const cab_page_cache* cache, int64_t n,
  * both are NULL. softmax over the seen tokens; a query that sees none and the queries past m
  * give 0 (lse -inf). lse [n,Hq,T] fp32 natural log, may be NULL. A sequence whose row is out
  * of range, whose m exceeds its length, or a page outside [0, pages) is not read: its output
- * is that of a query that sees none, or leaves out the page's tokens.
+ * is that of a query that sees none, or leaves out the page's tokens. width * page_size is at most
+ * 2^31 - 513.
  * bf16 / f16 with head_dim 64 or 128 and page_size 8, 16, 32, 64 or a multiple of 128 run on
  * the tensor cores (pages 16-byte aligned); other head_dim <= 256, page sizes and float32 on
  * CUDA cores.

@@ -25,3 +25,12 @@ def update(lib, c, dst=None, n=2, copies=1):
 def test_other_rows_without_copies(lib):
     assert update(lib, fake_cache(), dst=FAKE, copies=0) == 1
     assert b"copies" in lib.cab_last_error_string()
+
+
+@pytest.mark.parametrize("page,width,ok", [(16, (1 << 27) - 2, False), (16, (1 << 27) - 33, True),
+                                           (8, (1 << 28) - 2, False), (128, (1 << 24) - 5, True)])
+def test_rows_whose_tiles_would_pass_31_bits(lib, page, width, ok):
+    """Tile arithmetic rounds a row's length up to tiles of 128 and looks two tiles ahead."""
+    size = _lib._c_size(0)
+    c = fake_cache(page_size=page, width=width, table_stride=width)
+    assert lib.cab_tree_attn_workspace_size(c, 1, 4, 1, ctypes.byref(size)) == (0 if ok else 2)
