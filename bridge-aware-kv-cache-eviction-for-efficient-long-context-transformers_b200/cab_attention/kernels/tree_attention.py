@@ -20,7 +20,7 @@ import torch
 
 from .. import _lib
 
-_current_device = torch._C._cuda_getDevice  # the device is initialised: the tensors are on it
+_current_device = getattr(torch._C, "_cuda_getDevice", None)  # none in a torch without CUDA, where no call gets this far
 _INTS, _BOOLS = (torch.int32, torch.int64), (torch.bool, torch.uint8)
 
 
