@@ -165,7 +165,9 @@ class PagedKVCache:
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, num_new: Optional[torch.Tensor] = None,
               rows: Optional[torch.Tensor] = None) -> None:
         """Keys and values ``[n, Hkv, T, D]`` of each row's newest ``num_new`` (default T) tokens; tokens
-        t >= num_new[i] are not written. Rows must differ."""
+        t >= num_new[i] are not written. Rows must differ. Tokens that ``extend`` has made room for are in pages
+        of the row alone; older ones may be in pages that rows share, and are then written for all of them (by the
+        last of the sequences, where several do)."""
         if k.dim() != 4 or k.shape != v.shape or k.dtype is not self.dtype or v.dtype is not self.dtype:
             raise ValueError(f"k and v must be [n, Hkv, T, D] of the cache's dtype {self.dtype}")
         if k.device != self.device or v.device != self.device:

@@ -595,11 +595,17 @@ __global__ void __launch_bounds__(kWriteThreads, 3) write_kernel(const __grid_co
     RowSpan s{0, 0, -1, -1};
     if (t < w.m) {
       const int64_t pos = w.len - w.m + t, slot = pos % S;
-      const int64_t pg = c.block_table[w.row * c.table_stride + pos / S];
+      const int64_t col = pos / S, pg = c.block_table[w.row * c.table_stride + col];
+      const bool shared = c.ref_counts[pg] > 1;
       s.ksrc = (i * p.ks[0] + h * p.ks[1] + t * p.ks[2]) / vec_elems;
       s.vsrc = (i * p.vs[0] + h * p.vs[1] + t * p.vs[2]) / vec_elems;
       s.kdst = (p.layer * c.k_strides[0] + pg * c.k_strides[1] + h * c.k_strides[2] + slot * c.k_strides[3]) / vec_elems;
       s.vdst = (p.layer * c.v_strides[0] + pg * c.v_strides[1] + h * c.v_strides[2] + slot * c.v_strides[3]) / vec_elems;
+      // Rows share a page in the same column. Of several that write a token of it the last one does.
+      for (int j = shared ? i + 1 : p.n; j < p.n; ++j) {
+        const WriteRow o = write_row(p, j);
+        if (pos >= o.len - o.m && pos < o.len && c.block_table[o.row * c.table_stride + col] == pg) s.kdst = -1;
+      }
     }
     const int count = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(32), w.m - 32 * g)));
     move_rows<V>(static_cast<const V*>(p.k), static_cast<const V*>(p.v), static_cast<V*>(c.k_pages),

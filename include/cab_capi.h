@@ -376,7 +376,8 @@ CAB_API int cab_pages_update(const cab_page_cache* cache, const int32_t* src, co
 /*
  * Writes k, v [n,Hkv,T,D] (strides {n, h, t}, any non-negative) into one layer: token t of
  * sequence i, t < num_new[i] (NULL: num_value), becomes token seq_len - num_new[i] + t of row
- * rows[i] (NULL: i). Rows must differ. All or nothing: on a device-side refusal only the status
+ * rows[i] (NULL: i). Rows must differ. A token in a page that rows share is written for all of them;
+ * of several sequences that write it the last one counts. All or nothing: on a device-side refusal only the status
  * word changes.
  */
 CAB_API int cab_pages_write(const cab_page_cache* cache, int64_t layer, const void* k,
