@@ -205,7 +205,8 @@ class PagedKVCache:
 
     # ------------------------------------------------------------ host side
     def check(self) -> None:
-        """Waits for the device; raises (and clears) what it refused since the last check."""
+        """Waits for the device (all its streams); raises and clears what it refused since the last check."""
+        torch.cuda.synchronize(self.device)
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
@@ -213,4 +214,5 @@ class PagedKVCache:
 
     def free_pages(self) -> int:
         """Pages no row uses (waits for the device)."""
+        torch.cuda.synchronize(self.device)
         return int((self.ref_counts == 0).sum().item())

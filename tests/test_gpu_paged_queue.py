@@ -53,3 +53,19 @@ def test_attention_directly_after_a_change_of_lengths(S, D, lens):
     for _ in range(5):
         for x, y in zip(steps(False), want):
             assert torch.equal(x, y)
+
+
+def test_check_waits_for_calls_on_other_streams():
+    c, _ = make(P=20, R=3, W=6)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # about a tenth of a second
+        c.extend(20, dev([0]))
+    assert c.free_pages() == 18
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+        c.extend(1, dev([7]))
+    with pytest.raises(RuntimeError, match="outside the table"):
+        c.check()
+    c.check()
