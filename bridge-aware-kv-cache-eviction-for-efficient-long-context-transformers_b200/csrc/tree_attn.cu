@@ -1636,6 +1636,9 @@ extern "C" int cab_tree_attn_fwd(const cab_page_cache* cache, int64_t layer, con
   if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale)) return fail(CAB_ERR_INVALID_ARG, "tree_attn: softmax_scale must be > 0 and finite");
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] < 0 || o_strides[i] < 0) return fail(CAB_ERR_INVALID_ARG, "tree_attn: negative stride");
+  for (int i = 0; i < 3; ++i)
+    if (o_strides[i] == 0 && (i == 0 ? n : i == 1 ? Hq : T) > 1)
+      return fail(CAB_ERR_INVALID_ARG, "tree_attn: rows of the output in one place (stride 0)");
   const Layout L = layout(cache, n, Hq, T);
   if (L.total > 0 && (!workspace || workspace_bytes < L.total))
     return fail(CAB_ERR_WORKSPACE, "tree_attn: workspace of %zu bytes needed, %zu given", L.total, workspace_bytes);

@@ -34,3 +34,12 @@ def test_rows_whose_tiles_would_pass_31_bits(lib, page, width, ok):
     size = _lib._c_size(0)
     c = fake_cache(page_size=page, width=width, table_stride=width)
     assert lib.cab_tree_attn_workspace_size(c, 1, 4, 1, ctypes.byref(size)) == (0 if ok else 2)
+
+
+@pytest.mark.parametrize("strides", [(0, 1024, 64), (2048, 0, 64), (2048, 1024, 0)])
+def test_outputs_in_one_place(lib, strides):
+    """An expanded output: several rows would be stored over one another."""
+    s3 = _lib._i64_3(2048, 1024, 64)
+    rc = lib.cab_tree_attn_fwd(fake_cache(), 0, FAKE, FAKE, None, 2, 4, 2, s3, _lib._i64_3(*strides), None, None, None, 0, None,
+                               0, 0.1, FAKE, 1 << 30, None)
+    assert rc == 1 and b"output" in lib.cab_last_error_string()
