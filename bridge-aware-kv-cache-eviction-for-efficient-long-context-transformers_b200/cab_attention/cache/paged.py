@@ -42,7 +42,9 @@ class PagedKVCache:
     whose content ends inside it must belong to one row alone. ``allocate`` makes an empty cache.
 
     ``rows`` of a method (int32 or int64 ``[n]``, on the device; default: all rows in order) are table
-    rows; a call may change a row once. Counts may be given as a number or per row as a tensor."""
+    rows; a call may change a row once. Counts may be given as a number or per row as a tensor. A page update
+    (``extend``, ``truncate``, ``free``, ``fork``, ``compact``) takes at most 1024 rows: those of a larger cache
+    are listed in several calls."""
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
                  seq_lens: torch.Tensor, ref_counts: torch.Tensor, status: torch.Tensor):
@@ -140,7 +142,8 @@ class PagedKVCache:
         (any stride; default K): the eviction policy's ``keep`` and ``counts[:, 0]`` as they are, or the
         accepted nodes of a draft tree with ``start`` the context length. With ``dst`` the result becomes
         row ``dst[i]`` and row ``src[i]`` stays. Tokens that move are copied into fresh pages, so as many
-        pages as they fill must be free; pages whose tokens stay in place are kept or shared."""
+        pages as they fill must be free: for an eviction to ``budget`` tokens ``ceil(budget / page_size)`` for each
+        row of the call; pages whose tokens stay in place are kept or shared."""
         src, n = self._rows(src, "src")
         dst = int32_vector(dst, n, "dst", self.device)
         if start is None:

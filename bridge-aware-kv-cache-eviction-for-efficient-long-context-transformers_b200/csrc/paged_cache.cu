@@ -17,8 +17,8 @@
 // a page that drops to 0 can be taken by the next call, never by this one, since this call's
 // copies may still read it. Tokens R*S .. C-1 are then copied into the fresh pages.
 //
-// The update is all or nothing: every check is made before the first write, a refused call
-// changes nothing but the status word, and while the status word is set later calls do
+// Updates and writes are all or nothing: every check is made before the first store, a refused
+// call changes nothing but the status word, and while the status word is set later calls do
 // nothing either.
 
 #include "cab_host.h"
@@ -421,7 +421,8 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
 // comes from and goes to (three dependent small loads for 32 tokens at once), then the warp
 // moves the tokens' rows in vectors, kBatch loads of K and of V in flight per lane. Bound by
 // HBM: each moved value is read and written once. 2 x 6400 tokens of 8 heads of 128 kept out of 128,000:
-// 105 MB in 18 us, 5.8 TB/s; writing 2 x 32,768 tokens: 537 MB in 85 us, 6.3 TB/s (copy rate 6.55).
+// 105 MB in 18 us, 5.8 TB/s; writing 2 x 32,768 tokens: 537 MB in 88 us, 6.1 TB/s (copy rate 6.55), of
+// which 3 us are the checks before the first store.
 struct RowSpan {
   int64_t ksrc, vsrc, kdst, vdst;  // element offsets of a token's row
 };
