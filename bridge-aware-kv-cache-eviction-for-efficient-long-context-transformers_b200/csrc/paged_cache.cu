@@ -402,7 +402,8 @@ __global__ void __launch_bounds__(kUpdateThreads, 1) update_kernel(const __grid_
     for (int u = 0; u < kRound; ++u)
       if (write[u]) {
         const int i = pair[u], j = col[u];
-        if (j < s_had[i]) atomicSub(&c.ref_counts[gone[u]], 1);
+        // in range unless another stream changes the table during the call, where this is read a second time
+        if (j < s_had[i] && gone[u] >= 0 && gone[u] < P) atomicSub(&c.ref_counts[gone[u]], 1);
         if (page[u] >= 0) atomicAdd(&c.ref_counts[page[u]], 1);
         c.block_table[s_dst[i] * c.table_stride + j] = page[u];
         if (p.copies && page[u] >= 0 && j >= s_stay[i]) {
@@ -484,13 +485,15 @@ __global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ Updat
     RowSpan m{0, 0, -1, -1};
     if (lane < count) {
       const int pos = pos0 + lane;
-      const int from = pos < start ? pos : start + static_cast<int>(keep_at(p.keep, p.keep64, f.x * p.keep_stride + pos - start));
-      const int64_t pg = p.snap[static_cast<int64_t>(f.x) * c.width + from / S], slot = from % S;
-      const int64_t to = f.y, ts = 32 * g + lane;
+      const int64_t from = pos < start ? pos : start + keep_at(p.keep, p.keep64, f.x * p.keep_stride + pos - start);
+      // The list is read once more than it was checked: a stream that changes it meanwhile reaches nothing out of range.
+      const int64_t col = from >= 0 && from < c.width * S ? static_cast<int64_t>(static_cast<uint32_t>(from) / S) : -1;
+      const int64_t pg = col >= 0 ? p.snap[static_cast<int64_t>(f.x) * c.width + col] : -1, slot = from - col * S;
+      const int64_t to = pg >= 0 && pg < c.pages ? f.y : -1, ts = 32 * g + lane;
       const int64_t kb = l * c.k_strides[0] + h * c.k_strides[2], vb = l * c.v_strides[0] + h * c.v_strides[2];
       m.ksrc = (kb + pg * c.k_strides[1] + slot * c.k_strides[3]) / vec_elems;
       m.vsrc = (vb + pg * c.v_strides[1] + slot * c.v_strides[3]) / vec_elems;
-      m.kdst = (kb + to * c.k_strides[1] + ts * c.k_strides[3]) / vec_elems;
+      m.kdst = to < 0 ? -1 : (kb + to * c.k_strides[1] + ts * c.k_strides[3]) / vec_elems;
       m.vdst = (vb + to * c.v_strides[1] + ts * c.v_strides[3]) / vec_elems;
     }
     move_rows<V>(static_cast<const V*>(c.k_pages), static_cast<const V*>(c.v_pages), static_cast<V*>(c.k_pages),
@@ -594,18 +597,21 @@ __global__ void __launch_bounds__(kWriteThreads, 3) write_kernel(const __grid_co
     const WriteRow w = write_row(p, i);
     const int64_t t = 32 * g + lane;
     RowSpan s{0, 0, -1, -1};
-    if (t < w.m) {
-      const int64_t pos = w.len - w.m + t, slot = pos % S;
-      const int64_t col = pos / S, pg = c.block_table[w.row * c.table_stride + col];
-      const bool shared = c.ref_counts[pg] > 1;
-      s.ksrc = (i * p.ks[0] + h * p.ks[1] + t * p.ks[2]) / vec_elems;
-      s.vsrc = (i * p.vs[0] + h * p.vs[1] + t * p.vs[2]) / vec_elems;
-      s.kdst = (p.layer * c.k_strides[0] + pg * c.k_strides[1] + h * c.k_strides[2] + slot * c.k_strides[3]) / vec_elems;
-      s.vdst = (p.layer * c.v_strides[0] + pg * c.v_strides[1] + h * c.v_strides[2] + slot * c.v_strides[3]) / vec_elems;
-      // Rows share a page in the same column. Of several that write a token of it the last one does.
-      for (int j = shared ? i + 1 : p.n; j < p.n; ++j) {
-        const WriteRow o = write_row(p, j);
-        if (pos >= o.len - o.m && pos < o.len && c.block_table[o.row * c.table_stride + col] == pg) s.kdst = -1;
+    if (w.err == 0 && t < w.m) {
+      const int64_t pos = w.len - w.m + t, slot = pos % S, col = pos / S;
+      const int64_t pg = c.block_table[w.row * c.table_stride + col];
+      // The checks have passed. Should another stream change the cache all the same, nothing out of range is touched.
+      if (pg >= 0 && pg < c.pages) {
+        const bool shared = c.ref_counts[pg] > 1;
+        s.ksrc = (i * p.ks[0] + h * p.ks[1] + t * p.ks[2]) / vec_elems;
+        s.vsrc = (i * p.vs[0] + h * p.vs[1] + t * p.vs[2]) / vec_elems;
+        s.kdst = (p.layer * c.k_strides[0] + pg * c.k_strides[1] + h * c.k_strides[2] + slot * c.k_strides[3]) / vec_elems;
+        s.vdst = (p.layer * c.v_strides[0] + pg * c.v_strides[1] + h * c.v_strides[2] + slot * c.v_strides[3]) / vec_elems;
+        // Rows share a page in the same column. Of several that write a token of it the last one does.
+        for (int j = shared ? i + 1 : p.n; j < p.n; ++j) {
+          const WriteRow o = write_row(p, j);
+          if (o.err == 0 && pos >= o.len - o.m && pos < o.len && c.block_table[o.row * c.table_stride + col] == pg) s.kdst = -1;
+        }
       }
     }
     const int count = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(32), w.m - 32 * g)));

@@ -69,3 +69,39 @@ def test_check_waits_for_calls_on_other_streams():
     with pytest.raises(RuntimeError, match="outside the table"):
         c.check()
     c.check()
+
+
+@pytest.mark.parametrize("R,T", [(24, 3), (300, 5)])
+def test_captured_steps_with_idle_rows(R, T):
+    """extend, write, attend and truncate in one graph, replayed with other idle rows each time; 300 rows of 5 tokens
+    have more table entries than the write checks by itself."""
+    S, D, H = 4, 64, 2
+    c, _ = make(L=1, P=R * 80, H=H, S=S, D=D, R=R, W=80, seed=3)
+    lens = [130 + 7 * i % 150 for i in range(R)]
+    c.extend(dev(lens))
+    first = torch.randn(R, H, 280, D, device="cuda").to(torch.bfloat16)
+    c.write(0, first, first, dev(lens))
+    c.check()
+    k, q = (torch.randn(R, x, T, D, device="cuda").to(torch.bfloat16) for x in (H, 2 * H))
+    num, start = dev([T] * R), c.seq_lens.clone()
+
+    def step():
+        c.extend(num)
+        c.write(0, k, k, num)
+        out = c.attend(0, q, num_nodes=num, return_lse=True)
+        c.truncate(start)
+        return out
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for x in range(12):
+        num.copy_(dev([(T - i % 2 if (i + x) % 3 else 0) if x % 4 else T * ((i // 8 + x) % 2) for i in range(R)]))
+        want = [t.clone() for t in step()]
+        state = [t.clone() for t in (c.block_table, c.seq_lens, c.ref_counts)]
+        for _ in range(3):
+            graph.replay()
+            assert all(torch.equal(a, b) for a, b in zip(held, want))
+            assert all(torch.equal(a, b) for a, b in zip((c.block_table, c.seq_lens, c.ref_counts), state))
+    c.check()
